@@ -13,6 +13,7 @@ Produces, under ``forks-flash-mla-int_b200/lib/``:
 from __future__ import annotations
 
 import argparse
+import concurrent.futures
 import os
 import shutil
 import subprocess
@@ -25,7 +26,8 @@ CSRC = os.path.join(PKG, "csrc")
 LIB = os.path.join(PKG, "lib")
 INCLUDE = os.path.join(ROOT, "include")
 
-CUDA_SOURCES = ["sparse_mla_attn_sm100.cu", "quantize_int8_sm100.cu", "cache_writers_sm100.cu", "c_api.cu", "decode_static_scratch.cu"]
+CUDA_SOURCES = ["sparse_mla_attn_sm100.cu", "quantize_int8_sm100.cu", "cache_writers_sm100.cu",
+                "dense_prefill_sm100.cu", "row_weights_sm100.cu", "cache_eviction_sm100.cu", "c_api.cu", "decode_static_scratch.cu"]
 CUDA_HEADERS = ["sm100_ptx.cuh", "smla_internal.h", "row_codec.cuh"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
@@ -62,13 +64,21 @@ def build_core(force=False, verbose=False) -> str:
         os.path.join(INCLUDE, "sparse_mla_b200.h"), os.path.abspath(__file__)]
     if not force and _newer(out, deps):
         return out
-    cmd = [_nvcc(), "-O3", "-std=c++17", "-lineinfo", *ARCH, "-shared", "-Xcompiler", "-fPIC",
-           "-Xcompiler", "-fvisibility=hidden", "-I", INCLUDE, "-I", CSRC, "--expt-relaxed-constexpr",
-           "-cudart", "shared"]
+    # one object per source, compiled side by side; a header change recompiles all of them
+    flags = [_nvcc(), "-O3", "-std=c++17", "-lineinfo", *ARCH, "-Xcompiler", "-fPIC",
+             "-Xcompiler", "-fvisibility=hidden", "-I", INCLUDE, "-I", CSRC, "--expt-relaxed-constexpr"]
     if verbose:
-        cmd += ["-Xptxas", "-v"]
-    cmd += [os.path.join(CSRC, f) for f in CUDA_SOURCES] + ["-o", out]
-    _run(cmd, verbose)
+        flags += ["-Xptxas", "-v"]
+    headers = [os.path.join(CSRC, f) for f in CUDA_HEADERS] + [os.path.join(INCLUDE, "sparse_mla_b200.h"), os.path.abspath(__file__)]
+    objs, todo = [], []
+    for f in CUDA_SOURCES:
+        src, obj = os.path.join(CSRC, f), os.path.join(LIB, f.replace(".cu", ".o"))
+        objs.append(obj)
+        if force or not _newer(obj, [src] + headers):
+            todo.append([*flags, "-c", src, "-o", obj])
+    with concurrent.futures.ThreadPoolExecutor(max_workers=max(1, min(len(todo), os.cpu_count() or 1))) as pool:
+        list(pool.map(lambda c: _run(c, verbose), todo))
+    _run([_nvcc(), *ARCH, "-shared", "-cudart", "shared", *objs, "-o", out], verbose)
     return out
 
 

@@ -166,6 +166,90 @@ int smla_dense_mla_decode(const smla_dense_params_t *p, void *stream) {
     return smla::launch_dense_mla_attention(q, static_cast<cudaStream_t>(stream));
 }
 
+// The argument checks of these four come before the first CUDA call: they hold on a machine without a GPU too.
+int smla_dense_mla_prefill(const smla_prefill_params_t *p, void *stream) {
+    if (!p) return SMLA_EINVAL;
+    if (p->batch < 0 || p->total_q < 0 || p->total_k < 0 || p->num_heads <= 0 || p->num_kv_heads <= 0 ||
+        p->num_heads % p->num_kv_heads != 0 || (p->head_dim != 192 && p->head_dim != 128) || p->head_dim_v != 128 ||
+        p->dtype < 0 || p->dtype > 1 || !(p->softmax_scale == p->softmax_scale))
+        return SMLA_EINVAL;
+    if (p->batch == 0 || p->total_q == 0) return SMLA_OK;
+    if (!p->q || !p->out || !p->cu_seqlens_q || !p->cu_seqlens_k || (p->total_k > 0 && (!p->k || !p->v))) return SMLA_EINVAL;
+    if (p->total_q > 0x7FFFFFFFLL - 256 || p->total_k > 0x7FFFFFFFLL - 256 ||
+        (p->total_q / 256 + p->batch) * p->num_heads > 0x7FFFFFFFLL)
+        return SMLA_ETOOBIG;
+    const auto odd = [](const void *ptr, int64_t a, int64_t b) {
+        return (reinterpret_cast<uintptr_t>(ptr) & 15u) || (a & 7) || (b & 7);
+    };
+    if (odd(p->q, p->q_token_stride, p->q_head_stride) || odd(p->out, p->out_token_stride, p->out_head_stride) ||
+        (p->total_k > 0 && (odd(p->k, p->k_token_stride, p->k_head_stride) || odd(p->v, p->v_token_stride, p->v_head_stride))))
+        return SMLA_EALIGN;
+    DevInfo d;
+    const int rc = device_info(d);
+    if (rc != SMLA_OK) return rc;
+    if (d.major != 10) return SMLA_EARCH;
+    return smla::launch_dense_prefill(*p, d.sm_count, static_cast<cudaStream_t>(stream));
+}
+
+int smla_cache_row_weights(const smla_row_weights_params_t *p, void *stream) {
+    if (!p) return SMLA_EINVAL;
+    if (p->batch < 0 || p->seqlen_q <= 0 || p->num_heads <= 0 || (p->head_dim != 576 && p->head_dim != 512) ||
+        p->num_blocks < 0 || p->page_block_size <= 0 || p->max_blocks_per_seq < 0 || p->weights_width < 0 ||
+        p->block_table_stride < p->max_blocks_per_seq || p->weights_stride < p->weights_width ||
+        !(p->softmax_scale == p->softmax_scale))
+        return SMLA_EINVAL;
+    if (p->batch == 0 || p->weights_width == 0) return SMLA_OK;
+    if (!p->q || !p->softmax_lse || !p->cache_seqlens || !p->weights ||
+        (p->max_blocks_per_seq > 0 && (!p->block_table || (p->num_blocks > 0 && !p->k_cache))))
+        return SMLA_EINVAL;
+    if (static_cast<int64_t>(p->num_blocks) * p->page_block_size > 0x7FFFFFFFLL ||
+        static_cast<int64_t>(p->seqlen_q) * p->num_heads > 0x7FFFFFFFLL / 1024 ||
+        static_cast<int64_t>(p->batch) * p->seqlen_q * p->num_heads > 0x7FFFFFFFLL - 256)
+        return SMLA_ETOOBIG;
+    if ((reinterpret_cast<uintptr_t>(p->q) & 15u) || (reinterpret_cast<uintptr_t>(p->k_cache) & 15u) ||
+        (p->k_block_stride & 15) || (p->k_row_stride & 15) || p->k_row_stride < 2 * p->head_dim ||
+        p->page_block_size % 8 != 0)
+        return SMLA_EALIGN;
+    DevInfo d;
+    const int rc = device_info(d);
+    if (rc != SMLA_OK) return rc;
+    if (d.major != 10) return SMLA_EARCH;
+    return smla::launch_row_weights(*p, d.sm_count, static_cast<cudaStream_t>(stream));
+}
+
+int smla_select_cache_rows(const float *weights, int64_t weights_stride, int width, const int32_t *cache_seqlens,
+                           int batch, int budget, int recent, int32_t *rows, int32_t *kept, float *kept_weights,
+                           void *stream) {
+    if (batch < 0 || width < 0 || budget < 1 || recent < 0 || recent > budget || weights_stride < width) return SMLA_EINVAL;
+    if (batch == 0) return SMLA_OK;
+    if ((width > 0 && !weights) || !cache_seqlens || !rows || !kept) return SMLA_EINVAL;
+    DevInfo d;
+    const int rc = device_info(d);
+    if (rc != SMLA_OK) return rc;
+    if (d.major != 10) return SMLA_EARCH;
+    return smla::launch_select_rows(weights, weights_stride, width, cache_seqlens, batch, budget, recent, rows, kept,
+                                    kept_weights, static_cast<cudaStream_t>(stream));
+}
+
+int smla_compact_cache(const smla_compact_params_t *p, void *stream) {
+    if (!p) return SMLA_EINVAL;
+    if (p->batch < 0 || p->budget < 0 || p->row_bytes <= 0 || p->num_blocks < 0 || p->page_block_size <= 0 ||
+        p->max_blocks_per_seq < 0 || p->out_max_blocks_per_seq < 0 || p->block_table_stride < p->max_blocks_per_seq ||
+        p->out_block_table_stride < p->out_max_blocks_per_seq || p->row_stride < p->row_bytes)
+        return SMLA_EINVAL;
+    if (p->batch == 0 || p->budget == 0 || p->out_max_blocks_per_seq == 0 || p->num_blocks == 0) return SMLA_OK;
+    if (!p->cache || !p->out_block_table || !p->rows || !p->kept || (p->max_blocks_per_seq > 0 && !p->block_table))
+        return SMLA_EINVAL;
+    if ((reinterpret_cast<uintptr_t>(p->cache) & 15u) || (p->block_stride & 15) || (p->row_stride & 15) || (p->row_bytes & 15))
+        return SMLA_EALIGN;
+    if (static_cast<int64_t>(p->num_blocks) * p->page_block_size > 0x7FFFFFFFLL) return SMLA_ETOOBIG;
+    DevInfo d;
+    const int rc = device_info(d);
+    if (rc != SMLA_OK) return rc;
+    if (d.major != 10) return SMLA_EARCH;
+    return smla::launch_compact(*p, d.sm_count, static_cast<cudaStream_t>(stream));
+}
+
 int smla_sparse_mla_prefill(const smla_attn_params_t *p, void *stream) {
     if (!p) return SMLA_EINVAL;
     DevInfo d;

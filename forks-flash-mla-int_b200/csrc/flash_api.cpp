@@ -388,6 +388,207 @@ void fwd_kvcache_mla(const Tensor &q_in, const Tensor &kcache, const std::option
     check_rc(smla_dense_mla_decode(&p, current_stream(device)), "dense MLA decode");
 }
 
+// ------------------------------------------------------------------ dense prefill, eviction of cache rows
+// None of these ops has a counterpart in the reference; the names and the shapes follow the ops above.
+bool on_device(const Tensor &t, int device) { return t.is_cuda() && t.get_device_index() == device; }
+
+// [tokens, heads, dim] rows that the kernels can read with 16-byte loads and tensor copies (a dimension of size
+// one may carry any stride: it is never stepped over).
+bool usable_rows(const Tensor &t) {
+    return (t.size(2) <= 1 || t.stride(2) == 1) && (t.size(0) <= 1 || (t.stride(0) % 8 == 0 && t.stride(0) > 0)) &&
+           (t.size(1) <= 1 || (t.stride(1) % 8 == 0 && t.stride(1) > 0)) && aligned16(t);
+}
+int64_t token_stride(const Tensor &t) { return t.size(0) > 1 ? t.stride(0) : t.size(1) * t.size(2); }
+int64_t head_stride(const Tensor &t) { return t.size(1) > 1 ? t.stride(1) : t.size(2); }
+
+void dense_mla_prefill(const Tensor &q_in, const Tensor &k_in, const Tensor &v_in, const Tensor &cu_q_in, const Tensor &cu_k_in,
+                       double softmax_scale, bool causal, Tensor &out, Tensor &lse) {
+    STD_TORCH_CHECK(q_in.is_cuda(), "q must be on CUDA");
+    const int device = q_in.get_device_index();
+    STD_TORCH_CHECK(on_device(k_in, device) && on_device(v_in, device) && on_device(cu_q_in, device) && on_device(cu_k_in, device),
+                    "k, v, cu_seqlens_q and cu_seqlens_k must be on q's device");
+    STD_TORCH_CHECK(q_in.dim() == 3 && k_in.dim() == 3 && v_in.dim() == 3, "q, k and v must have shape (tokens, heads, dim)");
+    const auto type = q_in.scalar_type();
+    STD_TORCH_CHECK((type == ScalarType::BFloat16 || type == ScalarType::Half) && k_in.scalar_type() == type && v_in.scalar_type() == type,
+                    "q, k and v must be bfloat16, or all float16");
+    const int64_t TQ = q_in.size(0), H = q_in.size(1), D = q_in.size(2), TK = k_in.size(0), HK = k_in.size(1);
+    STD_TORCH_CHECK((D == 192 || D == 128) && k_in.size(2) == D && v_in.size(2) == 128, "head dims must be 192 or 128 for q and k, 128 for v");
+    STD_TORCH_CHECK(v_in.size(0) == TK && v_in.size(1) == HK, "k and v must have the same tokens and heads");
+    STD_TORCH_CHECK(H >= 1 && HK >= 1 && H % HK == 0, "the heads of q must be a multiple of the heads of k");
+    STD_TORCH_CHECK(cu_q_in.scalar_type() == ScalarType::Int && cu_k_in.scalar_type() == ScalarType::Int && cu_q_in.dim() == 1 &&
+                        cu_k_in.dim() == 1 && cu_q_in.size(0) >= 1 && cu_q_in.size(0) == cu_k_in.size(0),
+                    "cu_seqlens_q and cu_seqlens_k must be int32 tensors of shape (batch_size + 1,)");
+    torch::stable::accelerator::DeviceGuard guard(device);
+    const Tensor q = usable_rows(q_in) ? q_in : torch::stable::contiguous(torch::stable::clone(q_in));
+    const Tensor k = usable_rows(k_in) ? k_in : torch::stable::contiguous(torch::stable::clone(k_in));
+    const Tensor v = usable_rows(v_in) ? v_in : torch::stable::contiguous(torch::stable::clone(v_in));
+    const Tensor cu_q = cu_q_in.is_contiguous() ? cu_q_in : torch::stable::contiguous(cu_q_in);
+    const Tensor cu_k = cu_k_in.is_contiguous() ? cu_k_in : torch::stable::contiguous(cu_k_in);
+    out = torch::stable::new_empty(q, {TQ, H, 128});
+    lse = torch::stable::new_empty(q, {H, TQ}, ScalarType::Float);
+    STD_TORCH_CHECK(cu_q.size(0) - 1 <= 0x7FFFFFFF && H <= 0x7FFFFFFF, "too many sequences or heads");
+    smla_prefill_params_t p = {};
+    p.batch = static_cast<int32_t>(cu_q.size(0) - 1);
+    p.num_heads = static_cast<int32_t>(H);
+    p.num_kv_heads = static_cast<int32_t>(HK);
+    p.head_dim = static_cast<int32_t>(D);
+    p.head_dim_v = 128;
+    p.dtype = type == ScalarType::Half ? 1 : 0;
+    p.causal = causal ? 1 : 0;
+    p.softmax_scale = static_cast<float>(softmax_scale);
+    p.total_q = TQ;
+    p.total_k = TK;
+    p.q = q.data_ptr();
+    p.k = k.data_ptr();
+    p.v = v.data_ptr();
+    p.q_token_stride = token_stride(q);
+    p.q_head_stride = head_stride(q);
+    p.k_token_stride = token_stride(k);
+    p.k_head_stride = head_stride(k);
+    p.v_token_stride = token_stride(v);
+    p.v_head_stride = head_stride(v);
+    p.out = out.data_ptr();
+    p.out_token_stride = H * 128;
+    p.out_head_stride = 128;
+    p.softmax_lse = static_cast<float *>(lse.data_ptr());
+    p.lse_head_stride = TQ;
+    p.cu_seqlens_q = static_cast<const int32_t *>(cu_q.data_ptr());
+    p.cu_seqlens_k = static_cast<const int32_t *>(cu_k.data_ptr());
+    check_rc(smla_dense_mla_prefill(&p, current_stream(device)), "dense MLA prefill");
+}
+
+// A paged bf16 cache [num_blocks, page, 1, dim] with 16-byte aligned rows, and a block table beside it.
+void check_paged(const Tensor &cache, const Tensor &table, int device, int64_t batch, const char *what) {
+    STD_TORCH_CHECK(on_device(cache, device) && on_device(table, device), what, ": tensors must be on one CUDA device");
+    STD_TORCH_CHECK(cache.dim() == 4 && cache.size(2) == 1 && cache.scalar_type() == ScalarType::BFloat16 && cache.stride(3) == 1 &&
+                        cache.stride(0) % 8 == 0 && cache.stride(1) % 8 == 0 && cache.size(1) >= 1 && aligned16(cache) &&
+                        cache.size(0) * cache.size(1) <= 0x7FFFFFFF,
+                    what, ": k_cache must be a bfloat16 tensor (num_blocks, page_block_size, 1, head_size) with 16-byte aligned rows");
+    STD_TORCH_CHECK(table.scalar_type() == ScalarType::Int && table.dim() == 2 && table.size(0) == batch, what,
+                    ": block_table must be an int32 (batch_size, max_num_blocks_per_seq) tensor");
+}
+void check_lens(const Tensor &lens, int device, int64_t batch, const char *what) {
+    STD_TORCH_CHECK(on_device(lens, device) && lens.scalar_type() == ScalarType::Int && lens.dim() == 1 && lens.size(0) == batch, what,
+                    ": cache_seqlens must be an int32 (batch_size,) tensor on the same device");
+}
+// int32 [rows, columns] with unit column stride and rows in order
+Tensor as_table(const Tensor &t) {
+    return (t.size(1) <= 1 || t.stride(1) == 1) && (t.size(0) <= 1 || t.stride(0) >= t.size(1)) ? t : torch::stable::contiguous(torch::stable::clone(t));
+}
+int64_t row_stride_2d(const Tensor &t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
+
+// `weights` fp32 [batch, width] is added to when `accumulate`, else overwritten.
+void mla_cache_row_weights(const Tensor &q_in, const Tensor &cache, const Tensor &table_in, const Tensor &lens_in,
+                           const Tensor &lse_in, double softmax_scale, bool causal, const Tensor &weights, bool accumulate) {
+    const char *what = "MLA cache row weights";
+    STD_TORCH_CHECK(q_in.is_cuda() && q_in.dim() == 4 && q_in.scalar_type() == ScalarType::BFloat16, what,
+                    ": q must be a bfloat16 CUDA tensor (batch_size, seqlen_q, num_heads, head_size)");
+    const int device = q_in.get_device_index();
+    const int64_t B = q_in.size(0), SQ = q_in.size(1), H = q_in.size(2), D = q_in.size(3);
+    check_paged(cache, table_in, device, B, what);
+    check_lens(lens_in, device, B, what);
+    STD_TORCH_CHECK((D == 576 || D == 512) && cache.size(3) == D && SQ >= 1 && H >= 1, what, ": head_size must be 576 or 512 for q and k_cache");
+    STD_TORCH_CHECK(on_device(lse_in, device) && lse_in.scalar_type() == ScalarType::Float && lse_in.dim() == 3 && lse_in.size(0) == B &&
+                        lse_in.size(1) == H && lse_in.size(2) == SQ,
+                    what, ": softmax_lse must be a float32 (batch_size, num_heads, seqlen_q) tensor on q's device");
+    STD_TORCH_CHECK(on_device(weights, device) && weights.scalar_type() == ScalarType::Float && weights.dim() == 2 && weights.size(0) == B &&
+                        (weights.size(1) <= 1 || weights.stride(1) == 1) && (B <= 1 || weights.stride(0) >= weights.size(1)) &&
+                        weights.size(1) <= 0x7FFFFFFF,
+                    what, ": weights must be a float32 (batch_size, rows) tensor with contiguous rows on q's device");
+    torch::stable::accelerator::DeviceGuard guard(device);
+    const Tensor q = q_in.is_contiguous() && aligned16(q_in) ? q_in : torch::stable::contiguous(torch::stable::clone(q_in));
+    const Tensor lse = lse_in.is_contiguous() ? lse_in : torch::stable::contiguous(lse_in);
+    const Tensor lens = lens_in.is_contiguous() ? lens_in : torch::stable::contiguous(lens_in);
+    const Tensor table = as_table(table_in);
+    smla_row_weights_params_t p = {};
+    p.batch = static_cast<int32_t>(B);
+    p.seqlen_q = static_cast<int32_t>(SQ);
+    p.num_heads = static_cast<int32_t>(H);
+    p.causal = causal ? 1 : 0;
+    p.head_dim = static_cast<int32_t>(D);
+    p.softmax_scale = static_cast<float>(softmax_scale);
+    p.q = q.data_ptr();
+    p.softmax_lse = static_cast<const float *>(lse.data_ptr());
+    p.k_cache = cache.data_ptr();
+    p.k_row_stride = cache.size(1) > 1 ? cache.stride(1) * 2 : D * 2;
+    p.k_block_stride = cache.size(0) > 1 ? cache.stride(0) * 2 : p.k_row_stride * cache.size(1);
+    p.num_blocks = static_cast<int32_t>(cache.size(0));
+    p.page_block_size = static_cast<int32_t>(cache.size(1));
+    p.max_blocks_per_seq = static_cast<int32_t>(table.size(1));
+    p.block_table = static_cast<const int32_t *>(table.data_ptr());
+    p.block_table_stride = row_stride_2d(table);
+    p.cache_seqlens = static_cast<const int32_t *>(lens.data_ptr());
+    p.weights = static_cast<float *>(weights.data_ptr());
+    p.weights_width = static_cast<int32_t>(weights.size(1));
+    p.weights_stride = row_stride_2d(weights);
+    p.accumulate = accumulate ? 1 : 0;
+    check_rc(smla_cache_row_weights(&p, current_stream(device)), what);
+}
+
+void mla_select_cache_rows(const Tensor &weights_in, const Tensor &lens_in, int64_t budget, int64_t recent, Tensor &rows,
+                           Tensor &kept, Tensor &kept_weights) {
+    const char *what = "MLA cache row selection";
+    STD_TORCH_CHECK(weights_in.is_cuda() && weights_in.scalar_type() == ScalarType::Float && weights_in.dim() == 2, what,
+                    ": weights must be a float32 CUDA tensor (batch_size, rows)");
+    const int device = weights_in.get_device_index();
+    const int64_t B = weights_in.size(0);
+    check_lens(lens_in, device, B, what);
+    STD_TORCH_CHECK(budget >= 1 && budget <= 0x7FFFFFFF && recent >= 0 && recent <= budget, what, ": expected 0 <= recent <= budget and budget >= 1");
+    STD_TORCH_CHECK(weights_in.size(1) <= 0x7FFFFFFF && B <= 0x7FFFFFFF, what, ": too many rows");
+    torch::stable::accelerator::DeviceGuard guard(device);
+    const Tensor weights = as_table(weights_in);
+    const Tensor lens = lens_in.is_contiguous() ? lens_in : torch::stable::contiguous(lens_in);
+    rows = torch::stable::new_empty(lens, {B, budget});
+    kept = torch::stable::new_empty(lens, {B});
+    kept_weights = torch::stable::new_empty(weights, {B, budget});
+    check_rc(smla_select_cache_rows(static_cast<const float *>(weights.data_ptr()), row_stride_2d(weights), static_cast<int>(weights.size(1)),
+                                    static_cast<const int32_t *>(lens.data_ptr()), static_cast<int>(B), static_cast<int>(budget),
+                                    static_cast<int>(recent), static_cast<int32_t *>(rows.data_ptr()), static_cast<int32_t *>(kept.data_ptr()),
+                                    static_cast<float *>(kept_weights.data_ptr()), current_stream(device)),
+             what);
+}
+
+void mla_compact_cache(const Tensor &cache, const Tensor &table_in, const Tensor &rows_in, const Tensor &kept_in,
+                       const std::optional<Tensor> &out_table_in) {
+    const char *what = "MLA cache compaction";
+    STD_TORCH_CHECK(cache.is_cuda() && rows_in.dim() == 2, what, ": k_cache must be on CUDA, rows must have shape (batch_size, budget)");
+    const int device = cache.get_device_index();
+    const int64_t B = rows_in.size(0);
+    check_paged(cache, table_in, device, B, what);
+    check_lens(kept_in, device, B, what);
+    STD_TORCH_CHECK(on_device(rows_in, device) && rows_in.scalar_type() == ScalarType::Int, what, ": rows must be an int32 tensor on the same device");
+    STD_TORCH_CHECK(cache.size(3) % 8 == 0 && cache.size(3) >= 8, what, ": head_size must be a multiple of 8");
+    if (out_table_in.has_value()) check_paged(cache, out_table_in.value(), device, B, what);
+    torch::stable::accelerator::DeviceGuard guard(device);
+    const Tensor table = as_table(table_in);
+    // the caller's own table given as the target means a move in place, also where a copy of it had to be made
+    const bool in_place = !out_table_in.has_value() ||
+                          (out_table_in->data_ptr() == table_in.data_ptr() && out_table_in->size(1) == table_in.size(1) &&
+                           (B <= 1 || out_table_in->stride(0) == table_in.stride(0)) &&
+                           (table_in.size(1) <= 1 || out_table_in->stride(1) == table_in.stride(1)));
+    const Tensor out_table = in_place ? table : as_table(out_table_in.value());
+    const Tensor rows = rows_in.is_contiguous() ? rows_in : torch::stable::contiguous(rows_in);
+    const Tensor kept = kept_in.is_contiguous() ? kept_in : torch::stable::contiguous(kept_in);
+    smla_compact_params_t p = {};
+    p.batch = static_cast<int32_t>(B);
+    p.budget = static_cast<int32_t>(rows.size(1));
+    p.cache = cache.data_ptr();
+    p.row_bytes = static_cast<int32_t>(cache.size(3) * 2);
+    p.row_stride = cache.size(1) > 1 ? cache.stride(1) * 2 : cache.size(3) * 2;
+    p.block_stride = cache.size(0) > 1 ? cache.stride(0) * 2 : p.row_stride * cache.size(1);
+    p.num_blocks = static_cast<int32_t>(cache.size(0));
+    p.page_block_size = static_cast<int32_t>(cache.size(1));
+    p.block_table = static_cast<const int32_t *>(table.data_ptr());
+    p.block_table_stride = row_stride_2d(table);
+    p.max_blocks_per_seq = static_cast<int32_t>(table.size(1));
+    p.out_block_table = static_cast<const int32_t *>(out_table.data_ptr());
+    p.out_block_table_stride = row_stride_2d(out_table);
+    p.out_max_blocks_per_seq = static_cast<int32_t>(out_table.size(1));
+    p.rows = static_cast<const int32_t *>(rows.data_ptr());
+    p.kept = static_cast<const int32_t *>(kept.data_ptr());
+    check_rc(smla_compact_cache(&p, current_stream(device)), what);
+}
+
 // ------------------------------------------------------------------ boxed shims
 using torch::stable::detail::from;
 using torch::stable::detail::to;
@@ -472,6 +673,32 @@ void boxed_write_fp8(StableIValue *stack, uint64_t, uint64_t) {
                        to<Tensor>(stack[2]), 0);
 }
 
+void boxed_dense_prefill(StableIValue *stack, uint64_t, uint64_t) {
+    Tensor out, lse;
+    dense_mla_prefill(to<Tensor>(stack[0]), to<Tensor>(stack[1]), to<Tensor>(stack[2]), to<Tensor>(stack[3]), to<Tensor>(stack[4]),
+                      to<double>(stack[5]), to<bool>(stack[6]), out, lse);
+    stack[0] = from(out);
+    stack[1] = from(lse);
+}
+
+void boxed_row_weights(StableIValue *stack, uint64_t, uint64_t) {
+    mla_cache_row_weights(to<Tensor>(stack[0]), to<Tensor>(stack[1]), to<Tensor>(stack[2]), to<Tensor>(stack[3]), to<Tensor>(stack[4]),
+                          to<double>(stack[5]), to<bool>(stack[6]), to<Tensor>(stack[7]), to<bool>(stack[8]));
+}
+
+void boxed_select_rows(StableIValue *stack, uint64_t, uint64_t) {
+    Tensor rows, kept, kept_weights;
+    mla_select_cache_rows(to<Tensor>(stack[0]), to<Tensor>(stack[1]), to<int64_t>(stack[2]), to<int64_t>(stack[3]), rows, kept, kept_weights);
+    stack[0] = from(rows);
+    stack[1] = from(kept);
+    stack[2] = from(kept_weights);
+}
+
+void boxed_compact(StableIValue *stack, uint64_t, uint64_t) {
+    mla_compact_cache(to<Tensor>(stack[0]), to<Tensor>(stack[1]), to<Tensor>(stack[2]), to<Tensor>(stack[3]),
+                      to<std::optional<Tensor>>(stack[4]));
+}
+
 }  // namespace
 
 STABLE_TORCH_LIBRARY(flash_mla, m) {
@@ -497,6 +724,12 @@ STABLE_TORCH_LIBRARY(flash_mla, m) {
           "Tensor? extra_indices, Tensor? extra_lens, Tensor(a!) out, Tensor? workspace) -> ()");
     m.def("write_int8_ds_mla_cache(Tensor latent, Tensor slot_mapping, Tensor(a!) cache, int scale_rule) -> ()");
     m.def("write_fp8_ds_mla_cache(Tensor latent, Tensor slot_mapping, Tensor(a!) cache) -> ()");
+    m.def("dense_mla_prefill(Tensor q, Tensor k, Tensor v, Tensor cu_seqlens_q, Tensor cu_seqlens_k, float softmax_scale, "
+          "bool causal) -> (Tensor, Tensor)");
+    m.def("mla_cache_row_weights(Tensor q, Tensor kcache, Tensor block_table, Tensor cache_seqlens, Tensor softmax_lse, "
+          "float softmax_scale, bool causal, Tensor(a!) weights, bool accumulate) -> ()");
+    m.def("mla_select_cache_rows(Tensor weights, Tensor cache_seqlens, int budget, int recent) -> (Tensor, Tensor, Tensor)");
+    m.def("mla_compact_cache(Tensor(a!) kcache, Tensor block_table, Tensor rows, Tensor kept, Tensor? out_block_table) -> ()");
 }
 
 STABLE_TORCH_LIBRARY_IMPL(flash_mla, CUDA, m) {
@@ -510,6 +743,10 @@ STABLE_TORCH_LIBRARY_IMPL(flash_mla, CUDA, m) {
     m.impl("fwd_sparse_decode_mla_planned", &boxed_decode_planned);
     m.impl("write_int8_ds_mla_cache", &boxed_write_int8);
     m.impl("write_fp8_ds_mla_cache", &boxed_write_fp8);
+    m.impl("dense_mla_prefill", &boxed_dense_prefill);
+    m.impl("mla_cache_row_weights", &boxed_row_weights);
+    m.impl("mla_select_cache_rows", &boxed_select_rows);
+    m.impl("mla_compact_cache", &boxed_compact);
 }
 
 // `import flash_mla_cuda` only has to load this library so the static registrars above run.

@@ -19,6 +19,7 @@ SMLA_ETOOBIG = -5
 EXPORTS = (
     "smla_version", "smla_error_string", "smla_choose_num_splits", "smla_attn_workspace_bytes",
     "smla_decode_plan", "smla_decode_kernel_launches", "smla_decode_kernel_launches_captured", "smla_sparse_mla_decode", "smla_sparse_mla_decode_static_scratch", "smla_sparse_mla_prefill", "smla_dense_mla_decode",
+    "smla_dense_mla_prefill", "smla_cache_row_weights", "smla_select_cache_rows", "smla_compact_cache",
     "smla_quantize_int8_ds_mla_rows", "smla_write_int8_ds_mla_cache", "smla_write_fp8_ds_mla_cache",
     "smla_read_device_status", "smla_device_status_address",
 )
@@ -92,6 +93,84 @@ class SmlaDenseParams(C.Structure):
     ]
 
 
+class SmlaPrefillParams(C.Structure):
+    _fields_ = [
+        ("batch", C.c_int32),
+        ("num_heads", C.c_int32),
+        ("num_kv_heads", C.c_int32),
+        ("head_dim", C.c_int32),
+        ("head_dim_v", C.c_int32),
+        ("dtype", C.c_int32),
+        ("causal", C.c_int32),
+        ("softmax_scale", C.c_float),
+        ("total_q", C.c_int64),
+        ("total_k", C.c_int64),
+        ("q", C.c_void_p),
+        ("k", C.c_void_p),
+        ("v", C.c_void_p),
+        ("q_token_stride", C.c_int64),
+        ("q_head_stride", C.c_int64),
+        ("k_token_stride", C.c_int64),
+        ("k_head_stride", C.c_int64),
+        ("v_token_stride", C.c_int64),
+        ("v_head_stride", C.c_int64),
+        ("out", C.c_void_p),
+        ("out_token_stride", C.c_int64),
+        ("out_head_stride", C.c_int64),
+        ("softmax_lse", C.c_void_p),
+        ("lse_head_stride", C.c_int64),
+        ("cu_seqlens_q", C.c_void_p),
+        ("cu_seqlens_k", C.c_void_p),
+    ]
+
+
+class SmlaRowWeightsParams(C.Structure):
+    _fields_ = [
+        ("batch", C.c_int32),
+        ("seqlen_q", C.c_int32),
+        ("num_heads", C.c_int32),
+        ("causal", C.c_int32),
+        ("head_dim", C.c_int32),
+        ("softmax_scale", C.c_float),
+        ("q", C.c_void_p),
+        ("softmax_lse", C.c_void_p),
+        ("k_cache", C.c_void_p),
+        ("k_block_stride", C.c_int64),
+        ("k_row_stride", C.c_int64),
+        ("num_blocks", C.c_int32),
+        ("page_block_size", C.c_int32),
+        ("max_blocks_per_seq", C.c_int32),
+        ("block_table", C.c_void_p),
+        ("block_table_stride", C.c_int64),
+        ("cache_seqlens", C.c_void_p),
+        ("weights", C.c_void_p),
+        ("weights_stride", C.c_int64),
+        ("weights_width", C.c_int32),
+        ("accumulate", C.c_int32),
+    ]
+
+
+class SmlaCompactParams(C.Structure):
+    _fields_ = [
+        ("batch", C.c_int32),
+        ("budget", C.c_int32),
+        ("cache", C.c_void_p),
+        ("block_stride", C.c_int64),
+        ("row_stride", C.c_int64),
+        ("row_bytes", C.c_int32),
+        ("num_blocks", C.c_int32),
+        ("page_block_size", C.c_int32),
+        ("block_table", C.c_void_p),
+        ("block_table_stride", C.c_int64),
+        ("max_blocks_per_seq", C.c_int32),
+        ("out_block_table", C.c_void_p),
+        ("out_block_table_stride", C.c_int64),
+        ("out_max_blocks_per_seq", C.c_int32),
+        ("rows", C.c_void_p),
+        ("kept", C.c_void_p),
+    ]
+
+
 _lib = None
 
 
@@ -118,6 +197,11 @@ def load() -> C.CDLL:
     lib.smla_sparse_mla_prefill.argtypes = [C.POINTER(SmlaAttnParams), C.c_void_p]
     lib.smla_dense_mla_decode.argtypes = [C.POINTER(SmlaDenseParams), C.c_void_p]
     lib.smla_sparse_mla_decode_static_scratch.argtypes = [C.POINTER(SmlaAttnParams), C.c_void_p]
+    lib.smla_dense_mla_prefill.argtypes = [C.POINTER(SmlaPrefillParams), C.c_void_p]
+    lib.smla_cache_row_weights.argtypes = [C.POINTER(SmlaRowWeightsParams), C.c_void_p]
+    lib.smla_select_cache_rows.argtypes = [C.c_void_p, C.c_int64, C.c_int, C.c_void_p, C.c_int, C.c_int, C.c_int,
+                                           C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]
+    lib.smla_compact_cache.argtypes = [C.POINTER(SmlaCompactParams), C.c_void_p]
     lib.smla_quantize_int8_ds_mla_rows.argtypes = [C.c_void_p, C.c_int, C.c_int64, C.c_int64, C.c_void_p,
                                                    C.c_void_p, C.c_void_p]
     lib.smla_write_int8_ds_mla_cache.argtypes = [C.c_void_p, C.c_int, C.c_int64, C.c_int64, C.c_void_p, C.c_int,
@@ -199,4 +283,25 @@ def dense_params(q, k_cache, block_table, cache_seqlens, out, lse=None, softmax_
     if workspace is not None:
         p.workspace = workspace.data_ptr()
         p.workspace_bytes = workspace.numel() * workspace.element_size()
+    return p
+
+
+def prefill_params(q, k, v, cu_seqlens_q, cu_seqlens_k, out, lse=None, softmax_scale=None, causal=True) -> SmlaPrefillParams:
+    """q [total_q, h, 192 or 128], k [total_k, hk, .], v [total_k, hk, 128], out [total_q, h, 128] (bf16 or fp16), lse fp32
+    [h, total_q] or None."""
+    import torch
+    p = SmlaPrefillParams()
+    p.batch, p.num_heads, p.num_kv_heads = cu_seqlens_q.shape[0] - 1, q.shape[1], k.shape[1]
+    p.head_dim, p.head_dim_v = q.shape[2], v.shape[2]
+    p.dtype = 1 if q.dtype == torch.float16 else 0
+    p.causal = 1 if causal else 0
+    p.softmax_scale = softmax_scale if softmax_scale is not None else q.shape[-1] ** -0.5
+    p.total_q, p.total_k = q.shape[0], k.shape[0]
+    p.q, p.q_token_stride, p.q_head_stride = q.data_ptr(), q.stride(0), q.stride(1)
+    p.k, p.k_token_stride, p.k_head_stride = k.data_ptr(), k.stride(0), k.stride(1)
+    p.v, p.v_token_stride, p.v_head_stride = v.data_ptr(), v.stride(0), v.stride(1)
+    p.out, p.out_token_stride, p.out_head_stride = out.data_ptr(), out.stride(0), out.stride(1)
+    if lse is not None:
+        p.softmax_lse, p.lse_head_stride = lse.data_ptr(), lse.stride(0)
+    p.cu_seqlens_q, p.cu_seqlens_k = cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr()
     return p

@@ -193,6 +193,100 @@ typedef struct smla_dense_params {
 } smla_dense_params_t;
 SMLA_API int smla_dense_mla_decode(const smla_dense_params_t *params, void *stream);
 
+/* Dense MLA prefill: attention of whole prompts, packed one behind the other, over keys and values that have
+ * been expanded to heads (the decode above works on the latent rows instead).  Sequence b owns the query rows
+ * [cu_seqlens_q[b], cu_seqlens_q[b + 1]) and the key rows [cu_seqlens_k[b], cu_seqlens_k[b + 1]); with nq and nk
+ * of them, query i sees all nk keys or, with `causal`, the first nk - (nq - 1 - i): the queries are the
+ * sequence's last nq positions, so keys of an earlier part of the prompt may lie in front.  Query head h reads
+ * key head h / (num_heads / num_kv_heads).
+ *   out[i, h, :] = sum_j exp(scale q_i . k_j - lse_i) v_j,   lse[h, i] = log sum_j exp(scale q_i . k_j);
+ * a query that sees no key gets zeros and -inf.  Scores, statistics and sums are fp32; the weights are rounded
+ * to the input type in front of the second product.  Query rows outside every sequence are not written.
+ * Offsets that run backwards or past the totals are clamped: no row outside the buffers is touched.  A NaN or an
+ * infinity in a row of v reaches the queries of its own sequence only (also those that the mask hides it from).
+ * One launch, no workspace. */
+typedef struct smla_prefill_params {
+    int32_t batch;                        /* sequences                                                           */
+    int32_t num_heads, num_kv_heads;      /* num_heads a multiple of num_kv_heads                                */
+    int32_t head_dim, head_dim_v;         /* 192 or 128 for q and k; 128 for v and out                           */
+    int32_t dtype;                        /* 0 = bf16, 1 = fp16 (q, k, v and out)                                */
+    int32_t causal;
+    float softmax_scale;
+    int64_t total_q, total_k;             /* rows of q / out and of k / v, below 2^31                            */
+    const void *q, *k, *v;                /* 16-byte aligned                                                     */
+    int64_t q_token_stride, q_head_stride;       /* elements, multiples of 8                                    */
+    int64_t k_token_stride, k_head_stride;
+    int64_t v_token_stride, v_head_stride;
+    void *out;                            /* [total_q, num_heads, 128], 16-byte aligned                          */
+    int64_t out_token_stride, out_head_stride;
+    float *softmax_lse;                   /* fp32 [num_heads, total_q], natural log; may be NULL                 */
+    int64_t lse_head_stride;              /* elements                                                            */
+    const int32_t *cu_seqlens_q, *cu_seqlens_k;  /* [batch + 1]                                                  */
+} smla_prefill_params_t;
+SMLA_API int smla_dense_mla_prefill(const smla_prefill_params_t *params, void *stream);
+
+/* Eviction of cache rows by the attention they got, three calls.
+ *
+ * 1. smla_cache_row_weights: the weight of each cached row, summed over the heads and query positions of a call of
+ *    smla_dense_mla_decode with the same q, cache, table, lengths, scale and mask, from the log-sum-exp it returned:
+ *      w[b, r] = sum over i, h with r visible to query i of exp(scale q[b, i, h, :] . K[b, r, :] - lse[b, h, i]).
+ *    `accumulate` adds it to what `weights` holds for the rows of the sequence and leaves the others as they are;
+ *    without it the whole [batch, weights_width] is written, 0 behind the sequence's rows.  A query whose lse is
+ *    -inf gives nothing.  Sums are fp32 in a fixed order (two calls give the same bits).  A page number outside
+ *    the cache is a page of zero rows, as in the decode. */
+typedef struct smla_row_weights_params {
+    int32_t batch, seqlen_q, num_heads;   /* q [batch, seqlen_q, num_heads, head_dim] bf16                       */
+    int32_t causal;                       /* query position i sees the first len - (seqlen_q - 1 - i) rows       */
+    int32_t head_dim;                     /* 576 or 512                                                          */
+    float softmax_scale;
+    const void *q;                        /* 16-byte aligned; rows (b, i, h) head_dim elements apart, in order   */
+    const float *softmax_lse;             /* fp32 [batch, num_heads, seqlen_q], natural log, contiguous          */
+    const void *k_cache;                  /* [num_blocks, page_block_size, 1, head_dim] bf16, 16-byte aligned    */
+    int64_t k_block_stride, k_row_stride; /* bytes, multiples of 16, k_row_stride >= 2 * head_dim                */
+    int32_t num_blocks;
+    int32_t page_block_size;              /* a multiple of 8 (else SMLA_EALIGN)                                  */
+    int32_t max_blocks_per_seq;           /* columns of block_table: lengths are clamped to this many pages      */
+    const int32_t *block_table;           /* [batch, max_blocks_per_seq]                                         */
+    int64_t block_table_stride;           /* elements                                                            */
+    const int32_t *cache_seqlens;         /* [batch]                                                             */
+    float *weights;                       /* fp32 [batch, weights_width]                                         */
+    int64_t weights_stride;               /* elements between sequences                                          */
+    int32_t weights_width;                /* rows past it are left out                                           */
+    int32_t accumulate;
+} smla_row_weights_params_t;
+SMLA_API int smla_cache_row_weights(const smla_row_weights_params_t *params, void *stream);
+
+/* 2. smla_select_cache_rows: the rows of each sequence that stay when at most `budget` may.  All of them when the
+ *    length (clamped to `width`) is at most the budget; else the last `recent` rows and, of the rows in front of
+ *    them, the budget - recent with the largest weights, the lower row first where weights are equal (-0 equals
+ *    0, a NaN counts as less than every number).  rows[b, :kept[b]] ascend, -1 behind; kept_weights (may be NULL)
+ *    are their weights, 0 behind.  0 <= recent <= budget, budget >= 1. */
+SMLA_API int smla_select_cache_rows(const float *weights, int64_t weights_stride, int width,
+                                    const int32_t *cache_seqlens, int batch, int budget, int recent, int32_t *rows,
+                                    int32_t *kept, float *kept_weights, void *stream);
+
+/* 3. smla_compact_cache: row rows[b, j] of sequence b (through block_table) becomes its row j (through
+ *    out_block_table), j < kept[b].  rows [batch, budget] contiguous.  With out_block_table == block_table the rows
+ *    move inside their own pages: rows must then ascend, with rows[b, j] >= j (as selected above).  Otherwise the
+ *    pages written must not be among the pages read.  In both cases no page may be written for two sequences (or
+ *    twice for one).  A source row outside the table or the cache is a zero row; a target outside is left out.
+ *    row_bytes, strides and base are multiples of 16. */
+typedef struct smla_compact_params {
+    int32_t batch, budget;
+    void *cache;
+    int64_t block_stride, row_stride;     /* bytes                                                               */
+    int32_t row_bytes;
+    int32_t num_blocks, page_block_size;
+    const int32_t *block_table;
+    int64_t block_table_stride;           /* elements                                                            */
+    int32_t max_blocks_per_seq;
+    const int32_t *out_block_table;
+    int64_t out_block_table_stride;
+    int32_t out_max_blocks_per_seq;
+    const int32_t *rows, *kept;
+} smla_compact_params_t;
+SMLA_API int smla_compact_cache(const smla_compact_params_t *params, void *stream);
+
 /* int8_ds_mla row quantizer, bit-exact with quantize_int8_ds_mla_rows
  * (flash_mla/int8_sparse_mla.py:15-26): scale = max(amax|x|, 1e-12) / 127 and
  * q = clamp(rint(x / scale), -127, 127) in IEEE fp32.

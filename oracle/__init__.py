@@ -29,3 +29,5 @@ from .ds_mla_formats import (  # noqa: F401
 )
 from .sparse_mla_ref import sparse_mla_attention, cos_diff  # noqa: F401
 from .dense_mla_ref import dense_mla_decode  # noqa: F401
+from .dense_prefill_ref import dense_mla_prefill  # noqa: F401
+from .cache_eviction_ref import cache_row_weights, compact_cache, select_cache_rows, sequence_slots  # noqa: F401

@@ -1,0 +1,400 @@
+"""GPU tests of cache-row eviction: weights against the float64 oracle, selection and compaction exactly.
+
+Tolerance of the weights: each term exp(s - lse) is off by what its exponent is off, d 2^-23 scale sum |q k| for the
+dot product in fp32 plus 2^-22 of |s| and |lse| for scaling and subtraction, and by 2^-21 for the exponential; the sum of
+c terms adds c 2^-23 of itself.  The oracle returns sum term * (scale sum |q k| + |s| + |lse|), so the bound is
+(d + 4) 2^-23 times that plus (c 2^-23 + 2^-21) w.
+"""
+import ctypes
+import random
+
+import pytest
+import torch
+
+from helpers import device_status
+import oracle
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def fm():
+    import flash_mla
+    return flash_mla
+
+
+@pytest.fixture(autouse=True)
+def _status_clean():
+    yield
+    assert device_status() == 0, "a kernel wait ran out (device status word set)"
+
+
+def paged(lens, s_q=1, h=16, d=576, page=64, seed=0, extra=0, spare_columns=1):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    pages = [(n + page - 1) // page for n in lens]
+    perm = torch.randperm(sum(pages) + extra, generator=torch.Generator().manual_seed(seed)).to(torch.int32)
+    table = torch.full((len(lens), max(pages + [1]) + spare_columns), -1, dtype=torch.int32)
+    cache = torch.full((sum(pages) + extra + 1, page, 1, d), float("nan"), dtype=torch.bfloat16, device="cuda")
+    at = 0
+    for b, n in enumerate(lens):
+        table[b, :pages[b]] = perm[at:at + pages[b]]
+        at += pages[b]
+        rows = torch.full((pages[b] * page, d), float("nan"), device="cuda")
+        rows[:n] = torch.randn(n, d, generator=g, device="cuda")
+        cache[table[b, :pages[b]].long().cuda()] = rows.to(torch.bfloat16).view(pages[b], page, 1, d)
+    q = torch.randn(len(lens), s_q, h, d, generator=g, device="cuda").to(torch.bfloat16)
+    return dict(q=q, k_cache=cache, block_table=table.cuda(), cache_seqlens=torch.tensor(lens, dtype=torch.int32, device="cuda")), perm[at:]
+
+
+def lse_of(kw, causal, scale=None):
+    """log-sum-exp of the queries, in float64 on the host, as fp32."""
+    q, cache = kw["q"].cpu().double(), kw["k_cache"].cpu()
+    nb, page, _, d = cache.shape
+    b, sq, h, _ = q.shape
+    lse = torch.full((b, h, sq), float("-inf"), dtype=torch.float64)
+    table = kw["block_table"].cpu()
+    for i in range(b):
+        n = min(max(int(kw["cache_seqlens"][i]), 0), table.shape[1] * page)
+        if n == 0:
+            continue
+        pages = table[i].long()[torch.arange(n) // page]
+        rows = torch.zeros(n, d, dtype=torch.float64)
+        ok = (pages >= 0) & (pages < nb)
+        rows[ok] = cache[pages[ok], (torch.arange(n) % page)[ok], 0].double()
+        for t in range(sq):
+            see = n - (sq - 1 - t) if causal else n
+            if see > 0:
+                lse[i, :, t] = torch.logsumexp(rows[:see] @ q[i, t].T * (d ** -0.5 if scale is None else scale), dim=0)
+    return lse.float().cuda()
+
+
+def check_weights(got, kw, lse, causal, weights=None, scale=None, what=""):
+    ref, bound = oracle.cache_row_weights(kw["q"], kw["k_cache"], kw["block_table"], kw["cache_seqlens"], lse, scale=scale, causal=causal,
+                                          weights=weights, width=got.shape[1])
+    d, c = kw["q"].shape[3], kw["q"].shape[1] * kw["q"].shape[2]
+    tol = (d + 4) * 2.0 ** -23 * bound + (c * 2.0 ** -23 + 2.0 ** -21) * ref.abs() + 1e-30
+    w = got.cpu().double()
+    assert torch.isfinite(w).all(), f"{what}: non-finite weight"
+    bad = (w - ref).abs() - tol
+    assert bad.max() <= 0, f"{what}: off by {float((w - ref).abs().max()):.3e}, over the bound at {torch.nonzero(bad > 0)[:4].tolist()}"
+
+
+@pytest.mark.parametrize("d", [576, 512])
+@pytest.mark.parametrize("h", [1, 4, 16, 20, 32, 64, 128])
+@pytest.mark.parametrize("s_q", [1, 2, 5])
+def test_weights_heads_and_positions(fm, d, h, s_q):
+    kw, _ = paged([300, 1, 129, 64], s_q=s_q, h=h, d=d, seed=h + s_q)
+    lse = lse_of(kw, True)
+    got = fm.mla_cache_row_weights(**kw, softmax_lse=lse, causal=True)
+    assert got.shape == (4, kw["block_table"].shape[1] * 64)
+    check_weights(got, kw, lse, True, what=f"d={d} h={h} s_q={s_q}")
+
+
+@pytest.mark.parametrize("lens", [[1], [127], [128], [129], [255], [256], [257], [0, 3], [700, 0, 5], [1500]])
+@pytest.mark.parametrize("causal", [True, False])
+def test_weights_lengths(fm, lens, causal):
+    kw, _ = paged(lens, s_q=3, h=16, seed=len(lens))
+    lse = lse_of(kw, causal)
+    check_weights(fm.mla_cache_row_weights(**kw, softmax_lse=lse, causal=causal), kw, lse, causal, what=f"{lens}")
+
+
+@pytest.mark.parametrize("page", [8, 16, 24, 32, 48, 64, 96, 128, 256, 384])
+def test_weights_page_sizes(fm, page):
+    kw, _ = paged([500, 77], h=16, page=page, seed=page)
+    lse = lse_of(kw, False)
+    check_weights(fm.mla_cache_row_weights(**kw, softmax_lse=lse), kw, lse, False, what=f"page={page}")
+
+
+@pytest.mark.parametrize("s_q,h", [(40, 16), (16, 128), (33, 20), (64, 64)])
+def test_weights_of_a_window(fm, s_q, h):
+    """Hundreds to thousands of query columns; some sequences shorter than the window."""
+    kw, _ = paged([400, 20, 129], s_q=s_q, h=h, seed=s_q)
+    lse = lse_of(kw, True)
+    check_weights(fm.mla_cache_row_weights(**kw, softmax_lse=lse, causal=True), kw, lse, True, what=f"{s_q} x {h}")
+    lse = lse_of(kw, False)
+    check_weights(fm.mla_cache_row_weights(**kw, softmax_lse=lse, causal=False), kw, lse, False, what=f"{s_q} x {h} full")
+
+
+def test_weights_accumulate_into_views(fm):
+    kw, _ = paged([200, 130], s_q=2, h=16, seed=3)
+    lse = lse_of(kw, True)
+    g = torch.Generator(device="cuda").manual_seed(4)
+    for width in (150, 256, 300, 131):                       # narrower and wider than the sequences
+        buf = torch.rand(2, width + 5, generator=g, device="cuda")
+        w = buf[:, 3:3 + width]
+        before = w.clone()
+        got = fm.mla_cache_row_weights(**kw, softmax_lse=lse, causal=True, weights=w)
+        assert got.data_ptr() == w.data_ptr()
+        check_weights(got, kw, lse, True, weights=before, what=f"width {width}")
+        for b, n in enumerate((200, 130)):
+            assert torch.equal(w[b, min(n, width):], before[b, min(n, width):])
+        assert (buf[:, :3] != 0).all() and (buf[:, 3 + width:] != 0).all()
+
+
+def test_weights_from_the_lse_of_the_decode(fm):
+    """The decode's own lse: a query's weights sum to one (its scores round differently: 1e-3)."""
+    kw, _ = paged([900, 64, 333], s_q=2, h=16, seed=5)
+    meta, splits = fm.get_mla_metadata(kw["cache_seqlens"], 32, 1)
+    _, lse = fm.flash_mla_with_kvcache(kw["q"], kw["k_cache"], kw["block_table"], kw["cache_seqlens"], 512, meta, splits, causal=True)
+    w = fm.mla_cache_row_weights(**kw, softmax_lse=lse, causal=True)
+    check_weights(w, kw, lse, True)
+    assert (w.sum(1) - 32).abs().max() < 32e-3
+
+
+def test_weights_skip_queries_without_rows_and_bad_pages(fm):
+    kw, _ = paged([100, 200], s_q=2, h=4, seed=6)
+    lse = lse_of(kw, False)
+    lse[0, 1, 0] = float("-inf")
+    kw["block_table"][1, 1] = -5
+    kw["block_table"][1, 2] = 1 << 20
+    got = fm.mla_cache_row_weights(**kw, softmax_lse=lse)
+    check_weights(got, kw, lse, False)
+
+
+def test_weights_lengths_out_of_range(fm):
+    kw, _ = paged([100, 64], h=4, seed=7, spare_columns=0)
+    kw["cache_seqlens"] = torch.tensor([-3, 100000], dtype=torch.int32, device="cuda")
+    kw["k_cache"].nan_to_num_()
+    lse = lse_of(kw, False)
+    check_weights(fm.mla_cache_row_weights(**kw, softmax_lse=lse), kw, lse, False)
+
+
+def test_weights_strided_cache_table_and_q(fm):
+    kw, _ = paged([300, 40], s_q=2, h=8, d=512, seed=8)
+    wide = torch.full((kw["k_cache"].shape[0], 64, 1, 576 + 24), float("nan"), dtype=torch.bfloat16, device="cuda")
+    wide[..., :512] = kw["k_cache"]
+    kw["k_cache"] = wide[..., :512]
+    kw["block_table"] = torch.cat([kw["block_table"], torch.full_like(kw["block_table"], 3)], 1)[:, : kw["block_table"].shape[1]]
+    kw["q"] = kw["q"].transpose(1, 2).contiguous().transpose(1, 2)
+    lse = lse_of(kw, True)
+    check_weights(fm.mla_cache_row_weights(**kw, softmax_lse=lse, causal=True, softmax_scale=0.03), kw, lse, True, scale=0.03)
+
+
+def test_weights_many_sequences_same_bits_streams_and_graph(fm):
+    kw, _ = paged([(37 * i) % 300 for i in range(150)], h=16, seed=9)
+    lse = lse_of(kw, False)
+    one = fm.mla_cache_row_weights(**kw, softmax_lse=lse)
+    check_weights(one, kw, lse, False)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(torch.cuda.Stream()):
+        two = fm.mla_cache_row_weights(**kw, softmax_lse=lse)
+    torch.cuda.synchronize()
+    assert torch.equal(one, two)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        three = fm.mla_cache_row_weights(**kw, softmax_lse=lse)
+    kw["cache_seqlens"].copy_(kw["cache_seqlens"].flip(0).minimum(kw["cache_seqlens"]))
+    lse.copy_(lse_of(kw, False))
+    graph.replay()
+    torch.cuda.synchronize()
+    check_weights(three, kw, lse, False, what="replay")
+
+
+# ----------------------------------------------------------------------------- selection
+def same_selection(fm, w, lens, budget, recent):
+    got = fm.mla_select_cache_rows(w, lens, budget, recent)
+    ref = oracle.select_cache_rows(w, lens, budget, recent)
+    assert got[0].dtype == torch.int32 and got[1].dtype == torch.int32
+    assert torch.equal(got[1].cpu(), ref[1])
+    assert torch.equal(got[0].cpu(), ref[0]), f"budget {budget} recent {recent}"
+    assert torch.equal(got[2].cpu().view(torch.int32), ref[2].view(torch.int32))
+
+
+@pytest.mark.parametrize("budget,recent", [(1, 0), (1, 1), (7, 3), (64, 0), (64, 64), (500, 17), (2000, 100)])
+@pytest.mark.parametrize("width", [1, 33, 700, 1999])
+def test_select_sizes(fm, budget, recent, width):
+    g = torch.Generator(device="cuda").manual_seed(budget + width)
+    lens = torch.tensor([width, 0, max(1, width // 2), min(width, budget), min(width, budget + 1)], dtype=torch.int32, device="cuda")
+    w = torch.randn(5, width, generator=g, device="cuda").exp()
+    same_selection(fm, w, lens, budget, recent)
+
+
+def test_select_ties_signs_and_specials(fm):
+    g = torch.Generator(device="cuda").manual_seed(1)
+    base = torch.tensor([0.0, -0.0, 1.0, -1.0, float("inf"), float("-inf"), float("nan"), 1e-40, -1e-40, 3e38], device="cuda")
+    w = base[torch.randint(0, 10, (6, 1500), generator=g, device="cuda")]
+    w[4] = 0.0                                                # nothing but ties
+    w[5] = float("nan")
+    lens = torch.tensor([1500, 1499, 1000, 700, 1500, 1400], dtype=torch.int32, device="cuda")
+    for budget, recent in ((10, 0), (100, 33), (333, 1), (999, 0), (1499, 0)):
+        same_selection(fm, w, lens, budget, recent)
+
+
+def test_select_long_rows_and_views(fm):
+    g = torch.Generator(device="cuda").manual_seed(2)
+    buf = torch.rand(3, 140000, generator=g, device="cuda")
+    buf = torch.where(buf < 0.4, torch.zeros_like(buf), buf)
+    lens = torch.tensor([139990, 70001, 5000], dtype=torch.int32, device="cuda")
+    same_selection(fm, buf[:, 7:139997], lens, 9000, 128)
+    same_selection(fm, buf.t().contiguous().t(), lens, 333, 0)
+
+
+def test_select_very_long_row(fm):
+    g = torch.Generator(device="cuda").manual_seed(3)
+    w = torch.rand(1, 1_000_003, generator=g, device="cuda").mul(1 << 18).floor()
+    lens = torch.tensor([1_000_003], dtype=torch.int32, device="cuda")
+    rows, kept, vals = fm.mla_select_cache_rows(w, lens, 65536, 1000)
+    old = 1_000_003 - 1000
+    top = torch.sort(w[0, :old], descending=True, stable=True).indices[: 65536 - 1000].sort().values
+    ids = torch.cat([top, torch.arange(old, 1_000_003, device="cuda")])
+    assert torch.equal(rows[0].long(), ids) and int(kept) == 65536 and torch.equal(vals[0], w[0, ids])
+
+
+def test_select_lengths_out_of_range(fm):
+    w = torch.rand(3, 50, device="cuda")
+    same_selection(fm, w, torch.tensor([-7, 1000, 50], dtype=torch.int32, device="cuda"), 20, 5)
+    rows, kept, _ = fm.mla_select_cache_rows(w[:, :0], torch.tensor([1, 2, 3], dtype=torch.int32, device="cuda"), 4)
+    assert (rows == -1).all() and (kept == 0).all()
+
+
+def test_select_many_sequences_and_graph(fm):
+    g = torch.Generator(device="cuda").manual_seed(5)
+    w = torch.rand(400, 600, generator=g, device="cuda")
+    lens = torch.randint(0, 601, (400,), generator=g, device="cuda").to(torch.int32)
+    same_selection(fm, w, lens, 100, 20)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = fm.mla_select_cache_rows(w, lens, 100, 20)
+    w.copy_(torch.rand(400, 600, generator=g, device="cuda"))
+    graph.replay()
+    torch.cuda.synchronize()
+    for a, b in zip(got, oracle.select_cache_rows(w, lens, 100, 20)):
+        assert torch.equal(a.cpu(), b)
+
+
+# ----------------------------------------------------------------------------- compaction
+def same_bytes(a, b):
+    return torch.equal(a.cpu().view(torch.int16), b.cpu().view(torch.int16))
+
+
+def ascending(lens, budget, seed):
+    g = torch.Generator().manual_seed(seed)
+    rows = torch.full((len(lens), budget), -1, dtype=torch.int32)
+    for b, n in enumerate(lens):
+        m = min(n, budget)
+        rows[b, :m] = torch.randperm(n, generator=g)[:m].sort().values.to(torch.int32)
+    return rows.cuda(), torch.tensor([min(n, budget) for n in lens], dtype=torch.int32, device="cuda")
+
+
+@pytest.mark.parametrize("page", [1, 5, 16, 64, 100, 128])
+@pytest.mark.parametrize("d", [576, 512, 8, 40])
+@pytest.mark.parametrize("in_place", [True, False])
+def test_compact(fm, page, d, in_place):
+    lens, budget = [500, 3, 0, 129, 260], 120
+    per = (budget + page - 1) // page
+    kw, spare = paged(lens, h=1, d=d, page=page, seed=page + d, extra=0 if in_place else per * len(lens))
+    rows, kept = ascending(lens, budget, page)
+    out = None if in_place else spare.view(len(lens), per).cuda()
+    want = oracle.compact_cache(kw["k_cache"], kw["block_table"], rows, kept, out)
+    assert fm.mla_compact_cache(kw["k_cache"], kw["block_table"], rows, kept, out_block_table=out) is None
+    assert same_bytes(kw["k_cache"], want)
+
+
+def test_compact_long_in_place_and_own_table_as_target(fm):
+    lens = [20000, 9000]
+    for budget, given in ((12000, False), (19999, True), (300, False)):
+        kw, _ = paged(lens, h=1, d=64, page=16, seed=budget)
+        rows, kept = ascending(lens, budget, budget)
+        want = oracle.compact_cache(kw["k_cache"], kw["block_table"], rows, kept)
+        table = kw["block_table"]
+        if given:                                             # a strided table that the binding has to copy
+            table = torch.stack([table, table], 2)[:, :, 0]
+        fm.mla_compact_cache(kw["k_cache"], table, rows, kept, out_block_table=table if given else None)
+        assert same_bytes(kw["k_cache"], want)
+
+
+def test_compact_rows_and_pages_out_of_range(fm):
+    kw, spare = paged([100, 50], h=1, d=64, page=16, seed=1, extra=8)
+    rows = torch.tensor([[3, -4, 100000, 17], [49, 48, 47, 5]], dtype=torch.int32, device="cuda")     # any order into other pages
+    for kept in ([4, 4], [-2, 9], [2, 0]):
+        kept = torch.tensor(kept, dtype=torch.int32, device="cuda")
+        for out in (spare.view(2, 4)[:, :1], torch.tensor([[-1], [1 << 20]], dtype=torch.int32)):
+            cache = kw["k_cache"].clone()
+            want = oracle.compact_cache(cache, kw["block_table"], rows, kept, out)
+            fm.mla_compact_cache(cache, kw["block_table"], rows, kept, out_block_table=out.cuda().contiguous())
+            assert same_bytes(cache, want)
+    kw["block_table"][0, 0] = -1
+    cache = kw["k_cache"].clone()
+    kept = torch.tensor([4, 4], dtype=torch.int32, device="cuda")
+    want = oracle.compact_cache(cache, kw["block_table"], rows, kept, spare.view(2, 4)[:, :1])
+    fm.mla_compact_cache(cache, kw["block_table"], rows, kept, out_block_table=spare.view(2, 4)[:, :1].cuda())
+    assert same_bytes(cache, want)
+
+
+def test_compact_strided_cache_and_empty_calls(fm):
+    kw, _ = paged([70, 33], h=1, d=64, page=16, seed=2)
+    wide = torch.randn(kw["k_cache"].shape[0], 2, 16, 1, 96, device="cuda").to(torch.bfloat16)
+    wide[:, 1, :, :, :64] = kw["k_cache"]
+    view = wide[:, 1, :, :, :64]
+    rest = wide[:, 1, :, :, 64:].clone(), wide[:, 0].clone()
+    rows, kept = ascending([70, 33], 20, 3)
+    want = oracle.compact_cache(view, kw["block_table"], rows, kept)
+    fm.mla_compact_cache(view, kw["block_table"], rows, kept)
+    assert same_bytes(view.contiguous(), want)
+    assert torch.equal(wide[:, 1, :, :, 64:], rest[0]) and torch.equal(wide[:, 0], rest[1])
+    fm.mla_compact_cache(view, kw["block_table"], rows[:, :0], kept)
+    fm.mla_compact_cache(view, kw["block_table"][:0], rows[:0], kept[:0])
+    assert same_bytes(view.contiguous(), want)
+
+
+# ----------------------------------------------------------------------------- as they are used together
+def test_prompt_decode_evict_decode(fm):
+    """A small dense MLA layer: the prompt by prefill in the expanded form, its latent rows in the paged cache, a
+    decode step and the weights of its queries, eviction in place, and a decode over what stayed.  The prefill's
+    last position equals a decode of the same query in the absorbed form; the decode after the eviction equals
+    attention over the rows that were kept."""
+    torch.manual_seed(0)
+    dev, h, page, lens, budget, recent = "cuda", 16, 16, [130, 300, 40], 64, 16
+    total = sum(lens)
+    latent = torch.randn(total, 576, device=dev).to(torch.bfloat16)             # 512 latent + 64 rotary dims
+    w_k = (torch.randn(h, 128, 512, device=dev) / 512 ** 0.5).to(torch.bfloat16)
+    w_v = (torch.randn(h, 128, 512, device=dev) / 512 ** 0.5).to(torch.bfloat16)
+    q = torch.randn(total, h, 192, device=dev).to(torch.bfloat16)
+    scale = 192 ** -0.5
+    k = torch.cat([torch.einsum("tl,hnl->thn", latent[:, :512].float(), w_k.float()), latent[:, None, 512:].float().expand(-1, h, -1)], -1).to(torch.bfloat16)
+    v = torch.einsum("tl,hnl->thn", latent[:, :512].float(), w_v.float()).to(torch.bfloat16)
+    cu = torch.tensor([0, 130, 430, 470], dtype=torch.int32, device=dev)
+    out, lse = fm.dense_mla_prefill(q, k, v, cu, cu, softmax_scale=scale)
+
+    # the latent rows go to the pages; a decode of the last position must give the same as the prefill
+    per = 20
+    table = torch.randperm(3 * per).to(torch.int32).view(3, per).to(dev)
+    cache = torch.zeros(3 * per, page, 1, 576, dtype=torch.bfloat16, device=dev)
+    for b, n in enumerate(lens):
+        r = torch.arange(n, device=dev)
+        cache[table[b].long()[r // page], r % page, 0] = latent[cu[b]:cu[b + 1]]
+    seqlens = torch.tensor(lens, dtype=torch.int32, device=dev)
+    last = (cu[1:] - 1).long()
+
+    def absorbed(x):
+        return torch.cat([torch.einsum("bhn,hnl->bhl", x[..., :128].float(), w_k.float()), x[..., 128:].float()], -1).to(torch.bfloat16)[:, None]
+    meta, splits = fm.get_mla_metadata(seqlens, h, 1)
+    q_abs = absorbed(q[last])
+    o_abs, lse_dec = fm.flash_mla_with_kvcache(q_abs, cache, table, seqlens, 512, meta, splits, softmax_scale=scale, causal=True)
+    o_dec = torch.einsum("bhl,hnl->bhn", o_abs[:, 0].float(), w_v.float())
+    # k, v, absorbed q and the outputs are each rounded to bf16 on one of the two ways: a few 2^-8 of O(1) values
+    assert (o_dec - out[last].float()).abs().max() < 4 * 2.0 ** -8 * float(v.abs().max())
+    assert (lse_dec[:, :, 0] - lse[:, last].t()).abs().max() < 4 * 2.0 ** -8 * 10
+
+    weights = fm.mla_cache_row_weights(q_abs, cache, table, seqlens, lse_dec, softmax_scale=scale, causal=True)
+    assert (weights.sum(1) - h).abs().max() < 1e-2 * h
+    rows, kept, sums = fm.mla_select_cache_rows(weights, seqlens, budget, recent)
+    ref_rows, ref_kept, ref_sums = oracle.select_cache_rows(weights, seqlens, budget, recent)
+    assert torch.equal(rows.cpu(), ref_rows) and torch.equal(kept.cpu(), ref_kept) and torch.equal(sums.cpu(), ref_sums)
+    stay = [latent[cu[b]:cu[b + 1]][ref_rows[b, : int(ref_kept[b])].long().to(dev)] for b in range(3)]
+    fm.mla_compact_cache(cache, table, rows, kept)
+
+    meta, splits = fm.get_mla_metadata(kept, h, 1)
+    o2, lse2 = fm.flash_mla_with_kvcache(q_abs, cache, table, kept, 512, meta, splits, softmax_scale=scale, causal=True)
+    for b in range(3):
+        s = q_abs[b, 0].double() @ stay[b].double().t() * scale
+        ref = s.softmax(-1) @ stay[b][:, :512].double()
+        assert oracle.cos_diff(o2[b, 0].float().cpu().numpy(), ref.float().cpu().numpy()) < 8e-5
+        assert (lse2[b, :, 0].double() - s.logsumexp(-1)).abs().max() < 2e-3
+    # the sums go on: the rows that stayed keep what they had
+    acc = torch.zeros(3, per * page, device=dev)
+    acc[:, :budget] = sums
+    before = acc.clone()
+    fm.mla_cache_row_weights(q_abs, cache, table, kept, lse2, softmax_scale=scale, causal=True, weights=acc)
+    assert ((acc - before).sum(1) - h).abs().max() < 1e-2 * h
