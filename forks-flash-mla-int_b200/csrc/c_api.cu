@@ -200,7 +200,7 @@ int smla_cache_row_weights(const smla_row_weights_params_t *p, void *stream) {
         return SMLA_EINVAL;
     if (p->batch == 0 || p->weights_width == 0) return SMLA_OK;
     if (!p->q || !p->softmax_lse || !p->cache_seqlens || !p->weights ||
-        (p->max_blocks_per_seq > 0 && (!p->block_table || (p->num_blocks > 0 && !p->k_cache))))
+        !p->k_cache || p->num_blocks == 0 || (p->max_blocks_per_seq > 0 && !p->block_table))
         return SMLA_EINVAL;
     if (static_cast<int64_t>(p->num_blocks) * p->page_block_size > 0x7FFFFFFFLL ||
         static_cast<int64_t>(p->seqlen_q) * p->num_heads > 0x7FFFFFFFLL / 1024 ||

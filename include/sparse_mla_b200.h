@@ -243,7 +243,7 @@ typedef struct smla_row_weights_params {
     const float *softmax_lse;             /* fp32 [batch, num_heads, seqlen_q], natural log, contiguous          */
     const void *k_cache;                  /* [num_blocks, page_block_size, 1, head_dim] bf16, 16-byte aligned    */
     int64_t k_block_stride, k_row_stride; /* bytes, multiples of 16, k_row_stride >= 2 * head_dim                */
-    int32_t num_blocks;
+    int32_t num_blocks;                   /* at least 1                                                          */
     int32_t page_block_size;              /* a multiple of 8 (else SMLA_EALIGN)                                  */
     int32_t max_blocks_per_seq;           /* columns of block_table: lengths are clamped to this many pages      */
     const int32_t *block_table;           /* [batch, max_blocks_per_seq]                                         */
