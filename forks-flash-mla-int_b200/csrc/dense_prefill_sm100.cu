@@ -40,6 +40,9 @@ constexpr int kThreads = 384;
 constexpr int kSlab = 128 * 128;                 // bytes of [128 rows][64 dims] of 16-bit elements
 constexpr int kSlabs = 14;                       // Q and ring together
 constexpr int kRecords = 4;
+// Registers: 168 a thread at launch (the most that 384 threads can have); the softmax warps hold a row of 128 scores.
+constexpr int kRegsLaunch = 168, kRegsSoftmax = 208, kRegsOther = 88;
+static_assert(256 * kRegsSoftmax + 128 * kRegsOther <= kThreads * kRegsLaunch, "shares of the launch's registers");
 constexpr int kRecInts = 12;
 
 struct PrefillArgs {
@@ -416,19 +419,19 @@ __device__ __forceinline__ void softmax_role(const PrefillArgs &a, uint8_t *smem
             const uint64_t c2 = pack2(c, c), ref2 = pack2(ref, ref);
             uint64_t la = l2, lb = 0;
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                uint32_t w[32];
+            for (int j = 0; j < 4; ++j) {
+                uint32_t w[16];
 #pragma unroll
-                for (int e = 0; e < 32; ++e) {
+                for (int e = 0; e < 16; ++e) {
                     float x, y;
-                    unpack2(fma2(pack2(__uint_as_float(s[j * 64 + 2 * e]), __uint_as_float(s[j * 64 + 2 * e + 1])), c2, ref2), x, y);
+                    unpack2(fma2(pack2(__uint_as_float(s[j * 32 + 2 * e]), __uint_as_float(s[j * 32 + 2 * e + 1])), c2, ref2), x, y);
                     x = fast_exp2(x);
                     y = fast_exp2(y);
                     if (e & 1) lb = add2(lb, pack2(x, y));
                     else la = add2(la, pack2(x, y));
                     w[e] = pack16<FP16>(x, y);
                 }
-                tmem_st_x32(s_addr + j * 32, w);
+                tmem_st_x16(s_addr + j * 16, w);
             }
             l2 = add2(la, lb);
             tmem_st_wait();
@@ -508,9 +511,14 @@ __global__ void __launch_bounds__(kThreads, 1) dense_prefill_kernel(const __grid
     __syncthreads();
     tc_fence_after_sync();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(smem + L::kMisc + 8);
-    if (warp < 8) softmax_role<DQK, FP16>(a, smem, tmem, abort_flag, warp, lane);
-    else if (warp == 8) mma_role<DQK, FP16>(a, smem, tmem, abort_flag, lane);
-    else if (warp == 9) loader_role<DQK>(a, smem, abort_flag, lane);
+    if (warp < 8) {
+        regs_inc<kRegsSoftmax>();
+        softmax_role<DQK, FP16>(a, smem, tmem, abort_flag, warp, lane);
+    } else {
+        regs_dec<kRegsOther>();
+        if (warp == 8) mma_role<DQK, FP16>(a, smem, tmem, abort_flag, lane);
+        else if (warp == 9) loader_role<DQK>(a, smem, abort_flag, lane);
+    }
     tc_fence_before_sync();
     __syncthreads();
     if (warp == 8) {
@@ -522,7 +530,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_prefill_kernel(const __grid
 template <int DQK, bool FP16>
 int launch(PrefillArgs &a, unsigned grid, cudaStream_t stream) {
     static KernelSetup setup;
-    const int rc = setup.get(reinterpret_cast<const void *>(&dense_prefill_kernel<DQK, FP16>), Smem<DQK>::kBytes, &a.status);
+    const int rc = setup.get(reinterpret_cast<const void *>(&dense_prefill_kernel<DQK, FP16>), Smem<DQK>::kBytes, &a.status, kRegsLaunch);
     if (rc != 0) return rc;
     dense_prefill_kernel<DQK, FP16><<<grid, kThreads, Smem<DQK>::kBytes, stream>>>(a);
     return static_cast<int>(cudaGetLastError());

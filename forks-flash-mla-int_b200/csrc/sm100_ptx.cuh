@@ -119,6 +119,13 @@ __device__ __forceinline__ bool named_bar_or(int id, int nthreads, bool pred) {
     return r != 0;
 }
 
+// Registers per thread of this warpgroup (all four warps execute it).  An increase waits until the block's own pool,
+// launch registers x threads, has room: the shares of all warpgroups must not add up to more.
+template <int N>
+__device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
 // ----------------------------------------------------------------------------- tensor memory
 // Executed by one full warp.  ncols: power of two in [32, 512].
 __device__ __forceinline__ void tmem_alloc(uint32_t smem_dst, uint32_t ncols) {

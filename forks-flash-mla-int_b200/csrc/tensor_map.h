@@ -43,7 +43,8 @@ inline bool make_slab_map(CUtensorMap *map, bool fp16, const void *base, uint64_
 // The status word's address and the permission for `bytes` of shared memory, settled once per device and kernel.
 struct KernelSetup {
     std::atomic<int *> status[64] = {};
-    int get(const void *kernel, int bytes, int **status_out) {
+    // `regs`: registers per thread that the kernel must have been compiled to (it redistributes them; 0 = any)
+    int get(const void *kernel, int bytes, int **status_out, int regs = 0) {
         int dev = 0;
         cudaError_t e = cudaGetDevice(&dev);
         if (e != cudaSuccess) return static_cast<int>(e);
@@ -52,6 +53,10 @@ struct KernelSetup {
         if (s == nullptr) {
             e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
             if (e != cudaSuccess) return static_cast<int>(e);
+            cudaFuncAttributes attr;
+            e = cudaFuncGetAttributes(&attr, kernel);
+            if (e != cudaSuccess) return static_cast<int>(e);
+            if (attr.numRegs < regs) return static_cast<int>(cudaErrorInvalidKernelImage);
             const int rc = device_status_address(&s);
             if (rc != 0) return rc;
             if (tracked) status[dev].store(s, std::memory_order_release);
