@@ -185,7 +185,9 @@ __device__ __forceinline__ void loader_role(const PrefillArgs &a, uint8_t *smem,
         const int slot = it % kRecords;
         int *rec = reinterpret_cast<int *>(smem + L::kRecs) + slot * kRecInts;
         if (!(ok = mbar_wait(bars + (L::kBarRecEmpty + slot) * 8, ((it / kRecords) & 1) ^ 1, abort_flag))) break;
-        const bool more = find_item(a, w, blockIdx.x + static_cast<long long>(it) * gridDim.x, lane, rec);
+        // back and forth over the CTAs: the one with the largest item of a round gets the smallest of the next
+        const unsigned turn = (it & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x;
+        const bool more = find_item(a, w, static_cast<long long>(it) * gridDim.x + turn, lane, rec);
         if (!more && lane == 0) rec[kRecValid] = 0;
         __syncwarp();
         if (lane == 0) mbar_arrive(bars + (L::kBarRecFull + slot) * 8);
