@@ -3,13 +3,16 @@
 // Selection.  Weights become 32-bit keys that order as they do (sign folded, -0 made 0, NaN made the lowest).
 // Four passes of eight bits find the key T of the row that is last among the heaviest: a pass counts the
 // digits of the keys that agree with T so far and takes the digit at which the count from above reaches the
-// rows still wanted.  Rows above T stay, rows equal to T stay from the lowest on until the budget is full.
-// One CTA per sequence.
+// rows still wanted (and stops where a digit's rows are wanted all).  Rows above T stay, rows equal to T stay from
+// the lowest on until the budget is full, and all are written in row order by counting from the front.
+// Counts are integers, so nothing depends on the order of the atomics.
 //
-// Move.  Rows are copied in ascending order, a block of rows at a time: all loads of a block precede its
-// stores, so that in-place moves never overwrite a row that is still to be read (its source index is at
-// least its target's).
+// A cluster of CTAs takes a sequence.  Each holds its part of the keys in shared memory, so the weights are read
+// once, and the counts of a pass are added up through distributed shared memory.  What bounds it is latency: the four
+// passes, each a count, a cluster barrier and a search, one after the other.
+#include <cooperative_groups.h>
 #include <cuda_runtime.h>
+#include <algorithm>
 #include <cstdint>
 
 #include "smla_internal.h"
@@ -17,7 +20,11 @@
 namespace smla {
 namespace {
 
+namespace cg = cooperative_groups;
+
 constexpr int kSelThreads = 1024;
+constexpr int kSelWarps = kSelThreads / 32;
+constexpr int kMaxKeys = 48 * 1024;              // keys a CTA holds (192 KB); the rest is read again in each pass
 
 __device__ __forceinline__ uint32_t weight_key(float w) {
     if (w != w) return 0u;
@@ -25,120 +32,236 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
     return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-__global__ void __launch_bounds__(kSelThreads) select_rows_kernel(const float *weights, int64_t stride, int width,
-                                                                  const int32_t *lens, int budget, int recent, int32_t *rows,
-                                                                  int32_t *kept, float *kept_weights) {
-    __shared__ unsigned hist[256];
-    __shared__ unsigned s_prefix, s_want;
-    __shared__ int s_cnt[2][33];
-    const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int len = min(max(lens[b], 0), width);
+__global__ void __launch_bounds__(kSelThreads, 1) select_rows_kernel(const float *weights, int64_t stride, int width, const int32_t *lens,
+                                                                     int budget, int recent, int held, int32_t *rows, int32_t *kept,
+                                                                     float *kept_weights) {
+    extern __shared__ uint32_t keys[];           // `held` of this CTA's keys
+    __shared__ unsigned hist[2][256];
+    __shared__ unsigned total[256];
+    __shared__ int s_digit, s_left, s_all;
+    __shared__ int s_warp[2][kSelWarps];
+    __shared__ int s_sum[2];                     // this CTA's rows above T, and equal to it
+    cg::cluster_group cluster = cg::this_cluster();
+    const int ranks = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
+    const int b = blockIdx.x / ranks, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int len = min(max(lens[b], 0), width), stay = min(len, budget);
     const float *w = weights + b * stride;
     rows += static_cast<int64_t>(b) * budget;
     if (kept_weights) kept_weights += static_cast<int64_t>(b) * budget;
-    if (tid == 0) kept[b] = min(len, budget);
-    for (int j = min(len, budget) + tid; j < budget; j += kSelThreads) {
+    const int all = rank * kSelThreads + tid, step = ranks * kSelThreads;
+    if (all == 0) kept[b] = stay;
+    for (int j = stay + all; j < budget; j += step) {
         rows[j] = -1;
         if (kept_weights) kept_weights[j] = 0.0f;
     }
-    if (len <= budget) {
-        for (int j = tid; j < len; j += kSelThreads) {
-            rows[j] = j;
-            if (kept_weights) kept_weights[j] = w[j];
+    const int old = len - recent, want0 = budget - recent;   // of the `old` first rows `want0` stay
+    const bool whole = len <= budget;
+    if (whole || want0 == 0) {                   // (the whole cluster takes the same way)
+        const int first = whole ? 0 : old;
+        for (int j = all; j < stay; j += step) {
+            rows[j] = first + j;
+            if (kept_weights) kept_weights[j] = w[first + j];
         }
         return;
     }
-    const int old = len - recent, want0 = budget - recent;
-    for (int j = tid; j < recent; j += kSelThreads) {
+    for (int j = all; j < recent; j += step) {
         rows[want0 + j] = old + j;
         if (kept_weights) kept_weights[want0 + j] = w[old + j];
     }
-    if (want0 == 0) return;
+    // this CTA's part: whole multiples of 32 rows, in rank order
+    const int part = ((old + ranks - 1) / ranks + 31) & ~31;
+    const int lo = min(rank * part, old), n = min(part, old - lo);
+    w += lo;
+    const auto key_at = [&](int j) { return j < held ? keys[j] : weight_key(__ldg(w + j)); };
+    if (tid < 256) hist[0][tid] = hist[1][tid] = 0;
+    __syncthreads();
     unsigned prefix = 0, want = want0;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        if (tid < 256) hist[tid] = 0;
-        __syncthreads();
-        for (int j = tid; j < old; j += kSelThreads) {
-            const uint32_t k = weight_key(w[j]);
-            if (shift == 24 || (k >> (shift + 8)) == prefix) atomicAdd(&hist[(k >> shift) & 255], 1u);
+    int shift = 24;
+    for (int pass = 0;; ++pass, shift -= 8) {
+        unsigned *h = hist[pass & 1];
+        if (pass == 0) {
+#pragma unroll 4
+            for (int j = tid; j < n; j += kSelThreads) {
+                const uint32_t k = weight_key(__ldg(w + j));
+                if (j < held) keys[j] = k;
+                atomicAdd(&h[k >> 24], 1u);
+            }
+        } else {
+#pragma unroll 4
+            for (int j = tid; j < n; j += kSelThreads) {
+                const uint32_t k = key_at(j);
+                if ((k >> (shift + 8)) == prefix) atomicAdd(&h[(k >> shift) & 255], 1u);
+            }
+        }
+        if (ranks > 1) cluster.sync();
+        else __syncthreads();
+        if (tid < 256) {
+            unsigned sum = 0;
+            for (int r = 0; r < ranks; ++r) sum += *cluster.map_shared_rank(&h[tid], r);
+            total[tid] = sum;
+            hist[(pass & 1) ^ 1][tid] = 0;       // the other ranks have read it: they are past this pass's barrier
         }
         __syncthreads();
-        if (tid == 0) {
-            int d = 255;
-            unsigned left = want;
-            while (hist[d] < left) left -= hist[d--];
-            s_prefix = (prefix << 8) | d;
-            s_want = left;
+        if (warp == 0) {
+            // lane l has the digits 255 - 8 l down to 248 - 8 l; `above`: rows with larger digits than those
+            unsigned c[8], sum = 0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sum += c[e] = total[255 - 8 * lane - e];
+            unsigned upto = sum;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const unsigned x = __shfl_up_sync(0xffffffffu, upto, d);
+                if (lane >= d) upto += x;
+            }
+            unsigned above = upto - sum;
+            if (above < want && want <= upto) {  // one lane: the counts add up to at least `want`
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    if (above < want && want <= above + c[e]) {
+                        s_digit = 255 - 8 * lane - e;
+                        s_left = static_cast<int>(want - above);
+                        s_all = want - above == c[e];
+                    }
+                    above += c[e];
+                }
+            }
         }
         __syncthreads();
-        prefix = s_prefix;
-        want = s_want;
-        __syncthreads();
+        prefix = (prefix << 8) | static_cast<unsigned>(s_digit);
+        want = static_cast<unsigned>(s_left);
+        if (shift == 0 || s_all) break;
     }
-    // rows above `prefix` stay, and the first `want` rows equal to it
-    int out = 0, ties = 0;
-    for (int j0 = 0; j0 < old; j0 += kSelThreads) {
-        const int j = j0 + tid;
-        const uint32_t k = j < old ? weight_key(w[j]) : 0u;
-        const bool above = j < old && k > prefix, tie = j < old && k == prefix;
-        const unsigned ba = __ballot_sync(0xffffffffu, above), bt = __ballot_sync(0xffffffffu, tie);
-        if (lane == 0) {
-            s_cnt[0][warp] = __popc(ba);
-            s_cnt[1][warp] = __popc(bt);
-        }
-        __syncthreads();
-        int a = out, t = ties;
-        for (int i = 0; i < warp; ++i) {
-            a += s_cnt[0][i];
-            t += s_cnt[1][i];
-        }
-        for (int i = 0; i < kSelThreads / 32; ++i) {
-            out += s_cnt[0][i];
-            ties += s_cnt[1][i];
-        }
-        const unsigned below = (1u << lane) - 1u;
-        a += __popc(ba & below);
-        t += __popc(bt & below);
-        if (above || (tie && t < static_cast<int>(want))) {
-            const int at = a + min(t, static_cast<int>(want));
-            rows[at] = j;
-            if (kept_weights) kept_weights[at] = w[j];
-        }
-        __syncthreads();
+    // Rows whose key, without the bits not looked at, is above the prefix stay, and the first `want` that equal it.
+    const int warp_part = ((n + kSelWarps - 1) / kSelWarps + 31) & ~31;
+    const int w_lo = min(warp * warp_part, n), w_hi = min(w_lo + warp_part, n);
+    int above = 0, equal = 0;
+    for (int j = w_lo + lane; j < w_hi; j += 32) {
+        const uint32_t k = key_at(j) >> shift;
+        above += k > prefix;
+        equal += k == prefix;
     }
+    above = __reduce_add_sync(0xffffffffu, above);
+    equal = __reduce_add_sync(0xffffffffu, equal);
+    if (lane == 0) {
+        s_warp[0][warp] = above;
+        s_warp[1][warp] = equal;
+    }
+    __syncthreads();
+    if (warp == 0) {
+        const int a = s_warp[0][lane], t = s_warp[1][lane];
+        int ua = a, ut = t;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, ua, d), y = __shfl_up_sync(0xffffffffu, ut, d);
+            if (lane >= d) {
+                ua += x;
+                ut += y;
+            }
+        }
+        s_warp[0][lane] = ua - a;
+        s_warp[1][lane] = ut - t;
+        if (lane == 31) {
+            s_sum[0] = ua;
+            s_sum[1] = ut;
+        }
+    }
+    if (ranks > 1) cluster.sync();
+    else __syncthreads();
+    above = s_warp[0][warp];
+    equal = s_warp[1][warp];
+    for (int r = 0; r < rank; ++r) {
+        above += *cluster.map_shared_rank(&s_sum[0], r);
+        equal += *cluster.map_shared_rank(&s_sum[1], r);
+    }
+    const int ties = static_cast<int>(want);
+    const unsigned below = (1u << lane) - 1u;
+    for (int j0 = w_lo; j0 < w_hi; j0 += 32) {
+        const int j = j0 + lane;
+        const uint32_t k = j < w_hi ? key_at(j) >> shift : 0u;
+        const bool is_above = j < w_hi && k > prefix, is_equal = j < w_hi && k == prefix;
+        const unsigned ba = __ballot_sync(0xffffffffu, is_above), be = __ballot_sync(0xffffffffu, is_equal);
+        const int t = equal + __popc(be & below);
+        if (is_above || (is_equal && t < ties)) {
+            const int at = above + __popc(ba & below) + min(t, ties);
+            rows[at] = lo + j;
+            if (kept_weights) kept_weights[at] = __ldg(w + j);
+        }
+        above += __popc(ba);
+        equal += __popc(be);
+    }
+    if (ranks > 1) cluster.sync();               // no CTA may end while another reads its sums
 }
 
+// ------------------------------------------------------------------ move
 __device__ __forceinline__ const uint8_t *row_at(const smla_compact_params_t &p, const int32_t *table, int columns, int row) {
     const int col = row / p.page_block_size;
     if (row < 0 || col >= columns) return nullptr;
-    const int page = table[col];
+    const int page = __ldg(table + col);
     if (page < 0 || page >= p.num_blocks) return nullptr;
     return static_cast<const uint8_t *>(p.cache) + page * p.block_stride + (row - col * p.page_block_size) * p.row_stride;
 }
 
 constexpr int kMoveThreads = 256;
-constexpr int kSlice = 128;                                  // bytes of a row that one CTA moves
 
-__global__ void __launch_bounds__(kMoveThreads) compact_kernel(const smla_compact_params_t p) {
+// To other pages: every 16 bytes by themselves, consecutive threads on consecutive pieces of a row, four in flight per
+// thread.  Bound by HBM, 2 x row_bytes a row.
+constexpr int kMovePieces = 4;
+__global__ void __launch_bounds__(kMoveThreads) move_rows_kernel(const smla_compact_params_t p, int per_row) {
     const int b = blockIdx.y, n = min(max(p.kept[b], 0), p.budget);
-    const int piece = threadIdx.x % (kSlice / 16);
-    const int at = blockIdx.x * kSlice + piece * 16;
     const int32_t *rows = p.rows + static_cast<int64_t>(b) * p.budget;
-    constexpr int kRows = kMoveThreads / (kSlice / 16);
-    for (int j0 = 0; j0 < n; j0 += kRows) {
-        const int j = j0 + threadIdx.x / (kSlice / 16);
-        const bool mine = j < n && at < p.row_bytes;
-        uint4 x = make_uint4(0, 0, 0, 0);
-        if (mine) {
-            const uint8_t *src = row_at(p, p.block_table + b * p.block_table_stride, p.max_blocks_per_seq, rows[j]);
-            if (src) x = *reinterpret_cast<const uint4 *>(src + at);
+    const int32_t *from = p.block_table + b * p.block_table_stride, *to = p.out_block_table + b * p.out_block_table_stride;
+    const int64_t end = static_cast<int64_t>(n) * per_row;
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * (kMoveThreads * kMovePieces) + threadIdx.x;
+    uint4 x[kMovePieces];
+    uint8_t *dst[kMovePieces];
+#pragma unroll
+    for (int e = 0; e < kMovePieces; ++e) {
+        const int64_t i = first + e * kMoveThreads;
+        dst[e] = nullptr;
+        x[e] = make_uint4(0, 0, 0, 0);
+        if (i < end) {
+            const int j = static_cast<int>(static_cast<uint64_t>(i) <= 0xFFFFFFFFull ? static_cast<uint32_t>(i) / static_cast<uint32_t>(per_row) : i / per_row);
+            const int at = static_cast<int>(i - static_cast<int64_t>(j) * per_row) * 16;
+            const uint8_t *src = row_at(p, from, p.max_blocks_per_seq, __ldg(rows + j));
+            uint8_t *d = const_cast<uint8_t *>(row_at(p, to, p.out_max_blocks_per_seq, j));
+            if (src) x[e] = *reinterpret_cast<const uint4 *>(src + at);
+            if (d) dst[e] = d + at;
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < kMovePieces; ++e)
+        if (dst[e]) *reinterpret_cast<uint4 *>(dst[e]) = x[e];
+}
+
+// Inside their own pages: a CTA takes 64 bytes of all rows of a sequence (slices of a row do not touch one another) and
+// moves 512 rows at a time, all their loads in front of all their stores.  A row's source index is at least its target's,
+// so what a later turn reads has not been written yet.  Bound by the latency of a turn, a load and a barrier.
+constexpr int kSlice = 64, kSliceThreads = 512, kTurnRows = 512, kTurnPieces = kTurnRows / (kSliceThreads / (kSlice / 16));
+__global__ void __launch_bounds__(kSliceThreads) move_rows_in_place_kernel(const smla_compact_params_t p) {
+    const int b = blockIdx.y, n = min(max(p.kept[b], 0), p.budget);
+    const int at = blockIdx.x * kSlice + (threadIdx.x % (kSlice / 16)) * 16;
+    const int32_t *rows = p.rows + static_cast<int64_t>(b) * p.budget, *table = p.block_table + b * p.block_table_stride;
+    for (int j0 = 0; j0 < n; j0 += kTurnRows) {
+        uint4 x[kTurnPieces];
+#pragma unroll
+        for (int e = 0; e < kTurnPieces; ++e) {
+            const int j = j0 + e * (kTurnRows / kTurnPieces) + threadIdx.x / (kSlice / 16);
+            x[e] = make_uint4(0, 0, 0, 0);
+            if (j < n && at < p.row_bytes) {
+                const uint8_t *src = row_at(p, table, p.max_blocks_per_seq, __ldg(rows + j));
+                if (src) x[e] = *reinterpret_cast<const uint4 *>(src + at);
+            }
         }
         __syncthreads();
-        if (mine) {
-            uint8_t *dst = const_cast<uint8_t *>(row_at(p, p.out_block_table + b * p.out_block_table_stride, p.out_max_blocks_per_seq, j));
-            if (dst) *reinterpret_cast<uint4 *>(dst + at) = x;
+#pragma unroll
+        for (int e = 0; e < kTurnPieces; ++e) {
+            const int j = j0 + e * (kTurnRows / kTurnPieces) + threadIdx.x / (kSlice / 16);
+            if (j < n && at < p.row_bytes) {
+                uint8_t *dst = const_cast<uint8_t *>(row_at(p, table, p.max_blocks_per_seq, j));
+                if (dst) *reinterpret_cast<uint4 *>(dst + at) = x[e];
+            }
         }
-        __syncthreads();
+        __syncthreads();                         // the next turn's loads come behind these stores of the whole CTA
     }
 }
 
@@ -146,13 +269,41 @@ __global__ void __launch_bounds__(kMoveThreads) compact_kernel(const smla_compac
 
 int launch_select_rows(const float *weights, int64_t weights_stride, int width, const int32_t *lens, int batch, int budget,
                        int recent, int32_t *rows, int32_t *kept, float *kept_weights, cudaStream_t stream) {
-    select_rows_kernel<<<batch, kSelThreads, 0, stream>>>(weights, weights_stride, width, lens, budget, recent, rows, kept, kept_weights);
-    return static_cast<int>(cudaGetLastError());
+    // As many CTAs to a sequence as leave each at least 4096 rows and do not ask for more than one per SM (up to 8, the
+    // portable cluster size); more than 8 x 48 K rows are partly read from L2 in each pass.
+    int ranks = 1;
+    while (ranks < 8 && width / (ranks * 2) >= 4096 && static_cast<int64_t>(batch) * ranks * 2 <= 148) ranks *= 2;
+    while (ranks < 8 && width / ranks > kMaxKeys) ranks *= 2;
+    const int part = ((width + ranks - 1) / ranks + 31) & ~31, held = std::min(part, kMaxKeys);
+    if (static_cast<int64_t>(batch) * ranks > 0x7FFFFFFFLL) return SMLA_ETOOBIG;
+    cudaError_t e = cudaFuncSetAttribute(select_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxKeys * 4);
+    if (e != cudaSuccess) return static_cast<int>(e);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(batch) * ranks);
+    cfg.blockDim = dim3(kSelThreads);
+    cfg.dynamicSmemBytes = static_cast<size_t>(held) * 4;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = static_cast<unsigned>(ranks);
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, select_rows_kernel, weights, weights_stride, width, lens, budget, recent, held, rows, kept, kept_weights);
+    return static_cast<int>(e);
 }
 
 int launch_compact(const smla_compact_params_t &p, int, cudaStream_t stream) {
     if (p.batch > 65535) return SMLA_ETOOBIG;
-    compact_kernel<<<dim3((p.row_bytes + kSlice - 1) / kSlice, p.batch), kMoveThreads, 0, stream>>>(p);
+    if (p.out_block_table == p.block_table) {
+        move_rows_in_place_kernel<<<dim3(static_cast<unsigned>((p.row_bytes + kSlice - 1) / kSlice), static_cast<unsigned>(p.batch)), kSliceThreads, 0, stream>>>(p);
+    } else {
+        const int per_row = p.row_bytes / 16;
+        const int64_t pieces = static_cast<int64_t>(p.budget) * per_row, per_block = kMoveThreads * kMovePieces;
+        const int64_t blocks = (pieces + per_block - 1) / per_block;
+        if (blocks > 0x7FFFFFFFLL) return SMLA_ETOOBIG;
+        move_rows_kernel<<<dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(p.batch)), kMoveThreads, 0, stream>>>(p, per_row);
+    }
     return static_cast<int>(cudaGetLastError());
 }
 

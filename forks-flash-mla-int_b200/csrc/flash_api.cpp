@@ -392,6 +392,19 @@ void fwd_kvcache_mla(const Tensor &q_in, const Tensor &kcache, const std::option
 // None of these ops has a counterpart in the reference; the names and the shapes follow the ops above.
 bool on_device(const Tensor &t, int device) { return t.is_cuda() && t.get_device_index() == device; }
 
+// A contiguous tensor straight from the allocator: the dispatcher's way to it costs more than a small kernel's launch.
+Tensor empty_on(int device, std::initializer_list<int64_t> sizes, int32_t dtype) {
+    int64_t strides[4] = {1, 1, 1, 1}, n = 1;
+    const int64_t dims = static_cast<int64_t>(sizes.size());
+    for (int64_t i = dims - 1; i >= 0; --i) {
+        strides[i] = n;
+        n *= sizes.begin()[i] > 0 ? sizes.begin()[i] : 1;
+    }
+    AtenTensorHandle t = nullptr;
+    TORCH_ERROR_CODE_CHECK(aoti_torch_empty_strided(dims, sizes.begin(), strides, dtype, aoti_torch_device_type_cuda(), device, &t));
+    return Tensor(t);
+}
+
 // [tokens, heads, dim] rows that the kernels can read with 16-byte loads and tensor copies (a dimension of size
 // one may carry any stride: it is never stepped over).
 bool usable_rows(const Tensor &t) {
@@ -424,8 +437,8 @@ void dense_mla_prefill(const Tensor &q_in, const Tensor &k_in, const Tensor &v_i
     const Tensor v = usable_rows(v_in) ? v_in : torch::stable::contiguous(torch::stable::clone(v_in));
     const Tensor cu_q = cu_q_in.is_contiguous() ? cu_q_in : torch::stable::contiguous(cu_q_in);
     const Tensor cu_k = cu_k_in.is_contiguous() ? cu_k_in : torch::stable::contiguous(cu_k_in);
-    out = torch::stable::new_empty(q, {TQ, H, 128});
-    lse = torch::stable::new_empty(q, {H, TQ}, ScalarType::Float);
+    out = empty_on(device, {TQ, H, 128}, type == ScalarType::Half ? aoti_torch_dtype_float16() : aoti_torch_dtype_bfloat16());
+    lse = empty_on(device, {H, TQ}, aoti_torch_dtype_float32());
     STD_TORCH_CHECK(cu_q.size(0) - 1 <= 0x7FFFFFFF && H <= 0x7FFFFFFF, "too many sequences or heads");
     smla_prefill_params_t p = {};
     p.batch = static_cast<int32_t>(cu_q.size(0) - 1);
@@ -477,9 +490,9 @@ Tensor as_table(const Tensor &t) {
 }
 int64_t row_stride_2d(const Tensor &t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
 
-// `weights` fp32 [batch, width] is added to when `accumulate`, else overwritten.
-void mla_cache_row_weights(const Tensor &q_in, const Tensor &cache, const Tensor &table_in, const Tensor &lens_in,
-                           const Tensor &lse_in, double softmax_scale, bool causal, const Tensor &weights, bool accumulate) {
+// `given` fp32 [batch, width] is added to; without it a new tensor, a column for each row of the table, is filled.
+Tensor mla_cache_row_weights(const Tensor &q_in, const Tensor &cache, const Tensor &table_in, const Tensor &lens_in,
+                             const Tensor &lse_in, double softmax_scale, bool causal, const Tensor *given) {
     const char *what = "MLA cache row weights";
     STD_TORCH_CHECK(q_in.is_cuda() && q_in.dim() == 4 && q_in.scalar_type() == ScalarType::BFloat16, what,
                     ": q must be a bfloat16 CUDA tensor (batch_size, seqlen_q, num_heads, head_size)");
@@ -491,15 +504,19 @@ void mla_cache_row_weights(const Tensor &q_in, const Tensor &cache, const Tensor
     STD_TORCH_CHECK(on_device(lse_in, device) && lse_in.scalar_type() == ScalarType::Float && lse_in.dim() == 3 && lse_in.size(0) == B &&
                         lse_in.size(1) == H && lse_in.size(2) == SQ,
                     what, ": softmax_lse must be a float32 (batch_size, num_heads, seqlen_q) tensor on q's device");
-    STD_TORCH_CHECK(on_device(weights, device) && weights.scalar_type() == ScalarType::Float && weights.dim() == 2 && weights.size(0) == B &&
-                        (weights.size(1) <= 1 || weights.stride(1) == 1) && (B <= 1 || weights.stride(0) >= weights.size(1)) &&
-                        weights.size(1) <= 0x7FFFFFFF,
-                    what, ": weights must be a float32 (batch_size, rows) tensor with contiguous rows on q's device");
+    if (given) {
+        const Tensor &w = *given;
+        STD_TORCH_CHECK(on_device(w, device) && w.scalar_type() == ScalarType::Float && w.dim() == 2 && w.size(0) == B &&
+                            (w.size(1) <= 1 || w.stride(1) == 1) && (B <= 1 || w.stride(0) >= w.size(1)) && w.size(1) <= 0x7FFFFFFF,
+                        what, ": weights must be a float32 (batch_size, rows) tensor with contiguous rows on q's device");
+    }
+    STD_TORCH_CHECK(given || table_in.size(1) <= 0x7FFFFFFF / cache.size(1), what, ": block_table names too many rows");
     torch::stable::accelerator::DeviceGuard guard(device);
     const Tensor q = q_in.is_contiguous() && aligned16(q_in) ? q_in : torch::stable::contiguous(torch::stable::clone(q_in));
     const Tensor lse = lse_in.is_contiguous() ? lse_in : torch::stable::contiguous(lse_in);
     const Tensor lens = lens_in.is_contiguous() ? lens_in : torch::stable::contiguous(lens_in);
     const Tensor table = as_table(table_in);
+    const Tensor weights = given ? *given : empty_on(device, {B, table.size(1) * cache.size(1)}, aoti_torch_dtype_float32());
     smla_row_weights_params_t p = {};
     p.batch = static_cast<int32_t>(B);
     p.seqlen_q = static_cast<int32_t>(SQ);
@@ -521,8 +538,9 @@ void mla_cache_row_weights(const Tensor &q_in, const Tensor &cache, const Tensor
     p.weights = static_cast<float *>(weights.data_ptr());
     p.weights_width = static_cast<int32_t>(weights.size(1));
     p.weights_stride = row_stride_2d(weights);
-    p.accumulate = accumulate ? 1 : 0;
+    p.accumulate = given ? 1 : 0;
     check_rc(smla_cache_row_weights(&p, current_stream(device)), what);
+    return weights;
 }
 
 void mla_select_cache_rows(const Tensor &weights_in, const Tensor &lens_in, int64_t budget, int64_t recent, Tensor &rows,
@@ -538,9 +556,9 @@ void mla_select_cache_rows(const Tensor &weights_in, const Tensor &lens_in, int6
     torch::stable::accelerator::DeviceGuard guard(device);
     const Tensor weights = as_table(weights_in);
     const Tensor lens = lens_in.is_contiguous() ? lens_in : torch::stable::contiguous(lens_in);
-    rows = torch::stable::new_empty(lens, {B, budget});
-    kept = torch::stable::new_empty(lens, {B});
-    kept_weights = torch::stable::new_empty(weights, {B, budget});
+    rows = empty_on(device, {B, budget}, aoti_torch_dtype_int32());
+    kept = empty_on(device, {B}, aoti_torch_dtype_int32());
+    kept_weights = empty_on(device, {B, budget}, aoti_torch_dtype_float32());
     check_rc(smla_select_cache_rows(static_cast<const float *>(weights.data_ptr()), row_stride_2d(weights), static_cast<int>(weights.size(1)),
                                     static_cast<const int32_t *>(lens.data_ptr()), static_cast<int>(B), static_cast<int>(budget),
                                     static_cast<int>(recent), static_cast<int32_t *>(rows.data_ptr()), static_cast<int32_t *>(kept.data_ptr()),
@@ -682,8 +700,15 @@ void boxed_dense_prefill(StableIValue *stack, uint64_t, uint64_t) {
 }
 
 void boxed_row_weights(StableIValue *stack, uint64_t, uint64_t) {
+    Tensor w = mla_cache_row_weights(to<Tensor>(stack[0]), to<Tensor>(stack[1]), to<Tensor>(stack[2]), to<Tensor>(stack[3]),
+                                     to<Tensor>(stack[4]), to<double>(stack[5]), to<bool>(stack[6]), nullptr);
+    stack[0] = from(w);
+}
+
+void boxed_add_row_weights(StableIValue *stack, uint64_t, uint64_t) {
+    const Tensor weights = to<Tensor>(stack[7]);
     mla_cache_row_weights(to<Tensor>(stack[0]), to<Tensor>(stack[1]), to<Tensor>(stack[2]), to<Tensor>(stack[3]), to<Tensor>(stack[4]),
-                          to<double>(stack[5]), to<bool>(stack[6]), to<Tensor>(stack[7]), to<bool>(stack[8]));
+                          to<double>(stack[5]), to<bool>(stack[6]), &weights);
 }
 
 void boxed_select_rows(StableIValue *stack, uint64_t, uint64_t) {
@@ -727,7 +752,9 @@ STABLE_TORCH_LIBRARY(flash_mla, m) {
     m.def("dense_mla_prefill(Tensor q, Tensor k, Tensor v, Tensor cu_seqlens_q, Tensor cu_seqlens_k, float softmax_scale, "
           "bool causal) -> (Tensor, Tensor)");
     m.def("mla_cache_row_weights(Tensor q, Tensor kcache, Tensor block_table, Tensor cache_seqlens, Tensor softmax_lse, "
-          "float softmax_scale, bool causal, Tensor(a!) weights, bool accumulate) -> ()");
+          "float softmax_scale, bool causal) -> Tensor");
+    m.def("add_mla_cache_row_weights(Tensor q, Tensor kcache, Tensor block_table, Tensor cache_seqlens, Tensor softmax_lse, "
+          "float softmax_scale, bool causal, Tensor(a!) weights) -> ()");
     m.def("mla_select_cache_rows(Tensor weights, Tensor cache_seqlens, int budget, int recent) -> (Tensor, Tensor, Tensor)");
     m.def("mla_compact_cache(Tensor(a!) kcache, Tensor block_table, Tensor rows, Tensor kept, Tensor? out_block_table) -> ()");
 }
@@ -745,6 +772,7 @@ STABLE_TORCH_LIBRARY_IMPL(flash_mla, CUDA, m) {
     m.impl("write_fp8_ds_mla_cache", &boxed_write_fp8);
     m.impl("dense_mla_prefill", &boxed_dense_prefill);
     m.impl("mla_cache_row_weights", &boxed_row_weights);
+    m.impl("add_mla_cache_row_weights", &boxed_add_row_weights);
     m.impl("mla_select_cache_rows", &boxed_select_rows);
     m.impl("mla_compact_cache", &boxed_compact);
 }

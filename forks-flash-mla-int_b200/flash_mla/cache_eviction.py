@@ -22,6 +22,13 @@ from ._loader import load_torch_extension
 
 load_torch_extension()
 
+# The ops check their arguments themselves, in C++; the checks here are made when an op has refused, to say what is wrong
+# with a ValueError.  A small call is bound by the host, and checking twice would cost it several microseconds.
+_new_weights = torch.ops.flash_mla.mla_cache_row_weights.default
+_add_weights = torch.ops.flash_mla.add_mla_cache_row_weights.default
+_select = torch.ops.flash_mla.mla_select_cache_rows.default
+_compact = torch.ops.flash_mla.mla_compact_cache.default
+
 
 def _check_table(name: str, table: torch.Tensor, batch: int) -> None:
     if table.dim() != 2 or table.shape[0] != batch or table.dtype != torch.int32:
@@ -57,6 +64,18 @@ def mla_cache_row_weights(q: torch.Tensor, k_cache: torch.Tensor, block_table: t
             tensor with one column per row that ``block_table`` can name, 0 behind each length.
 
     Returns ``weights``.  The sums are formed in a fixed order: the same call gives the same bits."""
+    try:
+        scale = q.shape[-1] ** (-0.5) if softmax_scale is None else float(softmax_scale)
+        if weights is None:
+            return _new_weights(q, k_cache, block_table, cache_seqlens, softmax_lse, scale, causal)
+        _add_weights(q, k_cache, block_table, cache_seqlens, softmax_lse, scale, causal, weights)
+        return weights
+    except (RuntimeError, NotImplementedError, IndexError, ZeroDivisionError):
+        _check_weights_call(q, k_cache, block_table, cache_seqlens, softmax_lse, weights)
+        raise
+
+
+def _check_weights_call(q, k_cache, block_table, cache_seqlens, softmax_lse, weights) -> None:
     if q.dim() != 4 or q.shape[-1] not in (576, 512) or q.dtype != torch.bfloat16:
         raise ValueError(f"expected q bfloat16 [batch, seq_len_q, heads, 576 or 512], got {q.dtype} {tuple(q.shape)}")
     batch = q.shape[0]
@@ -72,14 +91,6 @@ def mla_cache_row_weights(q: torch.Tensor, k_cache: torch.Tensor, block_table: t
                          f"{tuple(softmax_lse.shape)}")
     if weights is not None and (weights.dim() != 2 or weights.shape[0] != batch or weights.dtype != torch.float32):
         raise ValueError(f"expected weights float32 [{batch}, rows], got {weights.dtype} {tuple(weights.shape)}")
-    if softmax_scale is None:
-        softmax_scale = q.shape[-1] ** (-0.5)
-    accumulate = weights is not None
-    if weights is None:
-        weights = torch.empty(batch, block_table.shape[1] * k_cache.shape[1], dtype=torch.float32, device=q.device)
-    torch.ops.flash_mla.mla_cache_row_weights(q, k_cache, block_table, cache_seqlens, softmax_lse, float(softmax_scale),
-                                              causal, weights, accumulate)
-    return weights
 
 
 def mla_select_cache_rows(weights: torch.Tensor, cache_seqlens: torch.Tensor, budget: int,
@@ -94,12 +105,15 @@ def mla_select_cache_rows(weights: torch.Tensor, cache_seqlens: torch.Tensor, bu
 
     Returns rows int32 (batch_size, budget), ascending, -1 behind the last; kept int32 (batch_size,), how many;
     kept_weights float32 (batch_size, budget), their weights, 0 behind."""
-    if weights.dim() != 2 or weights.dtype != torch.float32:
-        raise ValueError(f"expected weights float32 [batch, rows], got {weights.dtype} {tuple(weights.shape)}")
-    _check_lens("cache_seqlens", cache_seqlens, weights.shape[0])
-    if budget < 1 or not 0 <= recent <= budget:
-        raise ValueError(f"expected 0 <= recent <= budget and budget >= 1, got budget {budget}, recent {recent}")
-    return torch.ops.flash_mla.mla_select_cache_rows(weights, cache_seqlens, budget, recent)
+    try:
+        return _select(weights, cache_seqlens, budget, recent)
+    except (RuntimeError, NotImplementedError):
+        if weights.dim() != 2 or weights.dtype != torch.float32:
+            raise ValueError(f"expected weights float32 [batch, rows], got {weights.dtype} {tuple(weights.shape)}")
+        _check_lens("cache_seqlens", cache_seqlens, weights.shape[0])
+        if budget < 1 or not 0 <= recent <= budget:
+            raise ValueError(f"expected 0 <= recent <= budget and budget >= 1, got budget {budget}, recent {recent}")
+        raise
 
 
 def mla_compact_cache(k_cache: torch.Tensor, block_table: torch.Tensor, rows: torch.Tensor, kept: torch.Tensor,
@@ -114,14 +128,17 @@ def mla_compact_cache(k_cache: torch.Tensor, block_table: torch.Tensor, rows: to
 
     Arguments: k_cache bfloat16 (num_blocks, page_block_size, 1, head_dim), head_dim a multiple of 8; tables int32
     (batch_size, pages); rows int32 (batch_size, budget); kept int32 (batch_size,)."""
-    _check_cache(k_cache)
-    if rows.dim() != 2 or rows.dtype != torch.int32:
-        raise ValueError(f"expected rows int32 [batch, budget], got {rows.dtype} {tuple(rows.shape)}")
-    if k_cache.shape[3] % 8 != 0:
-        raise ValueError(f"expected a head_dim that is a multiple of 8, got {k_cache.shape[3]}")
-    batch = rows.shape[0]
-    _check_table("block_table", block_table, batch)
-    _check_lens("kept", kept, batch)
-    if out_block_table is not None:
-        _check_table("out_block_table", out_block_table, batch)
-    torch.ops.flash_mla.mla_compact_cache(k_cache, block_table, rows, kept, out_block_table)
+    try:
+        _compact(k_cache, block_table, rows, kept, out_block_table)
+    except (RuntimeError, NotImplementedError):
+        _check_cache(k_cache)
+        if rows.dim() != 2 or rows.dtype != torch.int32:
+            raise ValueError(f"expected rows int32 [batch, budget], got {rows.dtype} {tuple(rows.shape)}")
+        if k_cache.shape[3] % 8 != 0:
+            raise ValueError(f"expected a head_dim that is a multiple of 8, got {k_cache.shape[3]}")
+        batch = rows.shape[0]
+        _check_table("block_table", block_table, batch)
+        _check_lens("kept", kept, batch)
+        if out_block_table is not None:
+            _check_table("out_block_table", out_block_table, batch)
+        raise

@@ -15,6 +15,10 @@ from ._loader import load_torch_extension
 
 load_torch_extension()
 
+# The op checks its arguments itself, in C++; the checks below are made when it has refused, to say what is wrong with a
+# ValueError (a small call is bound by the host).
+_prefill = torch.ops.flash_mla.dense_mla_prefill.default
+
 
 def dense_mla_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens_q: torch.Tensor,
                       cu_seqlens_k: torch.Tensor, softmax_scale: Optional[float] = None,
@@ -37,6 +41,15 @@ def dense_mla_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seql
     Returns out (total_q, num_heads, 128) of q's type and softmax_lse (num_heads, total_q) float32, the natural
     logarithm of the sum of exponentials.  A query that sees no key gets zeros and -inf; rows of q behind the
     last sequence are not written."""
+    try:
+        scale = q.shape[-1] ** (-0.5) if softmax_scale is None else float(softmax_scale)
+        return _prefill(q, k, v, cu_seqlens_q, cu_seqlens_k, scale, causal)
+    except (RuntimeError, NotImplementedError, IndexError, ZeroDivisionError):
+        _check_call(q, k, v, cu_seqlens_q, cu_seqlens_k)
+        raise
+
+
+def _check_call(q, k, v, cu_seqlens_q, cu_seqlens_k) -> None:
     if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
         raise ValueError("expected q, k and v of shape [tokens, heads, head_dim]")
     if q.dtype not in (torch.bfloat16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:
@@ -52,6 +65,3 @@ def dense_mla_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seql
             raise ValueError(f"expected {name} int32 [batch + 1], got {cu.dtype} {tuple(cu.shape)}")
     if cu_seqlens_q.shape != cu_seqlens_k.shape:
         raise ValueError(f"cu_seqlens_q has {cu_seqlens_q.shape[0]} entries, cu_seqlens_k {cu_seqlens_k.shape[0]}")
-    if softmax_scale is None:
-        softmax_scale = q.shape[-1] ** (-0.5)
-    return torch.ops.flash_mla.dense_mla_prefill(q, k, v, cu_seqlens_q, cu_seqlens_k, float(softmax_scale), causal)
