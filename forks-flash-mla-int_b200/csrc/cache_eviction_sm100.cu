@@ -201,36 +201,42 @@ __device__ __forceinline__ const uint8_t *row_at(const smla_compact_params_t &p,
     return static_cast<const uint8_t *>(p.cache) + page * p.block_stride + (row - col * p.page_block_size) * p.row_stride;
 }
 
-constexpr int kMoveThreads = 256;
-
-// To other pages: every 16 bytes by themselves, consecutive threads on consecutive pieces of a row, four in flight per
-// thread.  Bound by HBM, 2 x row_bytes a row.
-constexpr int kMovePieces = 4;
-__global__ void __launch_bounds__(kMoveThreads) move_rows_kernel(const smla_compact_params_t p, int per_row) {
-    const int b = blockIdx.y, n = min(max(p.kept[b], 0), p.budget);
-    const int32_t *rows = p.rows + static_cast<int64_t>(b) * p.budget;
-    const int32_t *from = p.block_table + b * p.block_table_stride, *to = p.out_block_table + b * p.out_block_table_stride;
-    const int64_t end = static_cast<int64_t>(n) * per_row;
-    const int64_t first = static_cast<int64_t>(blockIdx.x) * (kMoveThreads * kMovePieces) + threadIdx.x;
-    uint4 x[kMovePieces];
-    uint8_t *dst[kMovePieces];
-#pragma unroll
-    for (int e = 0; e < kMovePieces; ++e) {
-        const int64_t i = first + e * kMoveThreads;
-        dst[e] = nullptr;
-        x[e] = make_uint4(0, 0, 0, 0);
-        if (i < end) {
-            const int j = static_cast<int>(static_cast<uint64_t>(i) <= 0xFFFFFFFFull ? static_cast<uint32_t>(i) / static_cast<uint32_t>(per_row) : i / per_row);
-            const int at = static_cast<int>(i - static_cast<int64_t>(j) * per_row) * 16;
-            const uint8_t *src = row_at(p, from, p.max_blocks_per_seq, __ldg(rows + j));
-            uint8_t *d = const_cast<uint8_t *>(row_at(p, to, p.out_max_blocks_per_seq, j));
-            if (src) x[e] = *reinterpret_cast<const uint4 *>(src + at);
-            if (d) dst[e] = d + at;
-        }
+// To other pages: a warp takes four rows, works out their addresses once and has all their pieces in flight together (three
+// of 16 bytes a lane and row: 1152 bytes are 2.25).  Bound by HBM, 2 x row_bytes a row.
+constexpr int kMoveWarps = 8, kMoveRows = 4, kMoveTurn = 3;
+__global__ void __launch_bounds__(kMoveWarps * 32) move_rows_kernel(const smla_compact_params_t p) {
+    const int b = blockIdx.y, n = min(max(__ldg(p.kept + b), 0), p.budget), lane = threadIdx.x & 31;
+    const int j0 = (blockIdx.x * kMoveWarps + (threadIdx.x >> 5)) * kMoveRows;
+    if (j0 >= n) return;
+    const uint8_t *src = nullptr;
+    uint8_t *dst = nullptr;
+    if (lane < kMoveRows && j0 + lane < n) {
+        const int row = __ldg(p.rows + static_cast<int64_t>(b) * p.budget + j0 + lane);
+        src = row_at(p, p.block_table + b * p.block_table_stride, p.max_blocks_per_seq, row);
+        dst = const_cast<uint8_t *>(row_at(p, p.out_block_table + b * p.out_block_table_stride, p.out_max_blocks_per_seq, j0 + lane));
     }
+    const uint8_t *from[kMoveRows];
+    uint8_t *to[kMoveRows];
 #pragma unroll
-    for (int e = 0; e < kMovePieces; ++e)
-        if (dst[e]) *reinterpret_cast<uint4 *>(dst[e]) = x[e];
+    for (int r = 0; r < kMoveRows; ++r) {
+        from[r] = reinterpret_cast<const uint8_t *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src), r));
+        to[r] = reinterpret_cast<uint8_t *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), r));
+    }
+    for (int at = lane * 16; at < p.row_bytes; at += kMoveTurn * 512) {
+        uint4 x[kMoveRows][kMoveTurn];
+#pragma unroll
+        for (int r = 0; r < kMoveRows; ++r)
+#pragma unroll
+            for (int e = 0; e < kMoveTurn; ++e) {
+                x[r][e] = make_uint4(0, 0, 0, 0);
+                if (from[r] && at + e * 512 < p.row_bytes) x[r][e] = __ldcs(reinterpret_cast<const uint4 *>(from[r] + at + e * 512));
+            }
+#pragma unroll
+        for (int r = 0; r < kMoveRows; ++r)
+#pragma unroll
+            for (int e = 0; e < kMoveTurn; ++e)
+                if (to[r] && at + e * 512 < p.row_bytes) *reinterpret_cast<uint4 *>(to[r] + at + e * 512) = x[r][e];
+    }
 }
 
 // Inside their own pages: a CTA takes 64 bytes of all rows of a sequence (slices of a row do not touch one another) and
@@ -298,11 +304,9 @@ int launch_compact(const smla_compact_params_t &p, int, cudaStream_t stream) {
     if (p.out_block_table == p.block_table) {
         move_rows_in_place_kernel<<<dim3(static_cast<unsigned>((p.row_bytes + kSlice - 1) / kSlice), static_cast<unsigned>(p.batch)), kSliceThreads, 0, stream>>>(p);
     } else {
-        const int per_row = p.row_bytes / 16;
-        const int64_t pieces = static_cast<int64_t>(p.budget) * per_row, per_block = kMoveThreads * kMovePieces;
-        const int64_t blocks = (pieces + per_block - 1) / per_block;
-        if (blocks > 0x7FFFFFFFLL) return SMLA_ETOOBIG;
-        move_rows_kernel<<<dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(p.batch)), kMoveThreads, 0, stream>>>(p, per_row);
+        constexpr int per_block = kMoveWarps * kMoveRows;
+        move_rows_kernel<<<dim3(static_cast<unsigned>((static_cast<int64_t>(p.budget) + per_block - 1) / per_block), static_cast<unsigned>(p.batch)),
+                           kMoveWarps * 32, 0, stream>>>(p);
     }
     return static_cast<int>(cudaGetLastError());
 }
