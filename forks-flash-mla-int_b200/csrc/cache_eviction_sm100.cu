@@ -35,9 +35,9 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 __global__ void __launch_bounds__(kSelThreads, 1) select_rows_kernel(const float *weights, int64_t stride, int width, const int32_t *lens,
                                                                      int budget, int recent, int held, int32_t *rows, int32_t *kept,
                                                                      float *kept_weights) {
-    extern __shared__ uint32_t keys[];           // `held` of this CTA's keys
+    extern __shared__ __align__(16) uint32_t keys[];         // `held` of this CTA's keys, a multiple of 4
     __shared__ unsigned hist[2][256];
-    __shared__ unsigned total[256];
+    __shared__ unsigned total[256];              // digit d at (255 - d) % 8 * 32 + (255 - d) / 8
     __shared__ int s_digit, s_left, s_all;
     __shared__ int s_warp[2][kSelWarps];
     __shared__ int s_sum[2];                     // this CTA's rows above T, and equal to it
@@ -64,15 +64,11 @@ __global__ void __launch_bounds__(kSelThreads, 1) select_rows_kernel(const float
         }
         return;
     }
-    for (int j = all; j < recent; j += step) {
-        rows[want0 + j] = old + j;
-        if (kept_weights) kept_weights[want0 + j] = w[old + j];
-    }
     // this CTA's part: whole multiples of 32 rows, in rank order
     const int part = ((old + ranks - 1) / ranks + 31) & ~31;
     const int lo = min(rank * part, old), n = min(part, old - lo);
-    w += lo;
-    const auto key_at = [&](int j) { return j < held ? keys[j] : weight_key(__ldg(w + j)); };
+    const float *mine = w + lo;
+    const auto key_at = [&](int j) { return j < held ? keys[j] : weight_key(__ldg(mine + j)); };
     if (tid < 256) hist[0][tid] = hist[1][tid] = 0;
     __syncthreads();
     unsigned prefix = 0, want = want0;
@@ -80,25 +76,33 @@ __global__ void __launch_bounds__(kSelThreads, 1) select_rows_kernel(const float
     for (int pass = 0;; ++pass, shift -= 8) {
         unsigned *h = hist[pass & 1];
         if (pass == 0) {
-#pragma unroll 4
+#pragma unroll 8
             for (int j = tid; j < n; j += kSelThreads) {
-                const uint32_t k = weight_key(__ldg(w + j));
+                const uint32_t k = weight_key(__ldg(mine + j));
                 if (j < held) keys[j] = k;
                 atomicAdd(&h[k >> 24], 1u);
             }
         } else {
-#pragma unroll 4
-            for (int j = tid; j < n; j += kSelThreads) {
-                const uint32_t k = key_at(j);
+            const auto count = [&](uint32_t k) {
                 if ((k >> (shift + 8)) == prefix) atomicAdd(&h[(k >> shift) & 255], 1u);
+            };
+            const int there = min(n, held) & ~3;
+#pragma unroll 2
+            for (int j = tid * 4; j < there; j += kSelThreads * 4) {
+                const uint4 k = *reinterpret_cast<const uint4 *>(keys + j);
+                count(k.x);
+                count(k.y);
+                count(k.z);
+                count(k.w);
             }
+            for (int j = there + tid; j < n; j += kSelThreads) count(key_at(j));
         }
         if (ranks > 1) cluster.sync();
         else __syncthreads();
         if (tid < 256) {
             unsigned sum = 0;
             for (int r = 0; r < ranks; ++r) sum += *cluster.map_shared_rank(&h[tid], r);
-            total[tid] = sum;
+            total[((255 - tid) & 7) * 32 + ((255 - tid) >> 3)] = sum;
             hist[(pass & 1) ^ 1][tid] = 0;       // the other ranks have read it: they are past this pass's barrier
         }
         __syncthreads();
@@ -106,7 +110,7 @@ __global__ void __launch_bounds__(kSelThreads, 1) select_rows_kernel(const float
             // lane l has the digits 255 - 8 l down to 248 - 8 l; `above`: rows with larger digits than those
             unsigned c[8], sum = 0;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) sum += c[e] = total[255 - 8 * lane - e];
+            for (int e = 0; e < 8; ++e) sum += c[e] = total[e * 32 + lane];
             unsigned upto = sum;
 #pragma unroll
             for (int d = 1; d < 32; d <<= 1) {
@@ -131,14 +135,39 @@ __global__ void __launch_bounds__(kSelThreads, 1) select_rows_kernel(const float
         want = static_cast<unsigned>(s_left);
         if (shift == 0 || s_all) break;
     }
-    // Rows whose key, without the bits not looked at, is above the prefix stay, and the first `want` that equal it.
-    const int warp_part = ((n + kSelWarps - 1) / kSelWarps + 31) & ~31;
+    // Rows whose key, without the bits not looked at, is above the prefix stay, and the first `want` that equal it.  A warp
+    // takes consecutive rows, a lane four of them at a time.
+    const int warp_part = ((n + kSelWarps - 1) / kSelWarps + 127) & ~127;
     const int w_lo = min(warp * warp_part, n), w_hi = min(w_lo + warp_part, n);
+    const auto four = [&](int j, uint32_t (&k)[4]) {         // keys of rows j .. j + 3, shifted, and which of them there are
+        if (j + 3 < min(n, held)) {
+            const uint4 x = *reinterpret_cast<const uint4 *>(keys + j);
+            k[0] = x.x >> shift;
+            k[1] = x.y >> shift;
+            k[2] = x.z >> shift;
+            k[3] = x.w >> shift;
+            return 0xFu;
+        }
+        unsigned have = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            k[e] = 0;
+            if (j + e < n) {
+                k[e] = key_at(j + e) >> shift;
+                have |= 1u << e;
+            }
+        }
+        return have;
+    };
     int above = 0, equal = 0;
-    for (int j = w_lo + lane; j < w_hi; j += 32) {
-        const uint32_t k = key_at(j) >> shift;
-        above += k > prefix;
-        equal += k == prefix;
+    for (int j = w_lo + lane * 4; j < w_hi; j += 128) {
+        uint32_t k[4];
+        const unsigned have = four(j, k);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            above += ((have >> e) & 1u) && k[e] > prefix;
+            equal += ((have >> e) & 1u) && k[e] == prefix;
+        }
     }
     above = __reduce_add_sync(0xffffffffu, above);
     equal = __reduce_add_sync(0xffffffffu, equal);
@@ -174,20 +203,46 @@ __global__ void __launch_bounds__(kSelThreads, 1) select_rows_kernel(const float
         equal += *cluster.map_shared_rank(&s_sum[1], r);
     }
     const int ties = static_cast<int>(want);
-    const unsigned below = (1u << lane) - 1u;
-    for (int j0 = w_lo; j0 < w_hi; j0 += 32) {
-        const int j = j0 + lane;
-        const uint32_t k = j < w_hi ? key_at(j) >> shift : 0u;
-        const bool is_above = j < w_hi && k > prefix, is_equal = j < w_hi && k == prefix;
-        const unsigned ba = __ballot_sync(0xffffffffu, is_above), be = __ballot_sync(0xffffffffu, is_equal);
-        const int t = equal + __popc(be & below);
-        if (is_above || (is_equal && t < ties)) {
-            const int at = above + __popc(ba & below) + min(t, ties);
-            rows[at] = lo + j;
-            if (kept_weights) kept_weights[at] = __ldg(w + j);
+    for (int j0 = w_lo; j0 < w_hi; j0 += 128) {
+        const int j = j0 + lane * 4;
+        uint32_t k[4];
+        const unsigned have = four(j, k);
+        unsigned is_above = 0, is_equal = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            is_above |= static_cast<unsigned>(k[e] > prefix) << e;
+            is_equal |= static_cast<unsigned>(k[e] == prefix) << e;
         }
-        above += __popc(ba);
-        equal += __popc(be);
+        is_above &= have;
+        is_equal &= have;
+        const int both = __popc(is_above) | (__popc(is_equal) << 16);
+        int upto = both;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, upto, d);
+            if (lane >= d) upto += x;
+        }
+        const int sum = __shfl_sync(0xffffffffu, upto, 31), front = upto - both;
+        int a = above + (front & 0xFFFF), t = equal + (front >> 16);
+        if (is_above | is_equal) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const bool up = (is_above >> e) & 1u, tie = (is_equal >> e) & 1u;
+                if (up || (tie && t < ties)) {
+                    const int at = a + min(t, ties);
+                    rows[at] = lo + j + e;
+                    if (kept_weights) kept_weights[at] = __ldg(mine + j + e);
+                }
+                a += up;
+                t += tie;
+            }
+        }
+        above += sum & 0xFFFF;
+        equal += sum >> 16;
+    }
+    for (int j = all; j < recent; j += step) {
+        rows[want0 + j] = old + j;
+        if (kept_weights) kept_weights[want0 + j] = w[old + j];
     }
     if (ranks > 1) cluster.sync();               // no CTA may end while another reads its sums
 }
