@@ -217,6 +217,15 @@ int smla_cache_row_weights(const smla_row_weights_params_t *p, void *stream) {
     return smla::launch_row_weights(*p, d.sm_count, static_cast<cudaStream_t>(stream));
 }
 
+int smla_cache_row_weights_workspace(int seqlen_q, int num_heads, size_t *bytes) {
+    if (!bytes || seqlen_q <= 0 || num_heads <= 0) return SMLA_EINVAL;
+    DevInfo d;
+    const int rc = device_info(d);
+    if (rc != SMLA_OK) return rc;
+    *bytes = smla::row_weights_workspace(seqlen_q, num_heads, d.sm_count);
+    return SMLA_OK;
+}
+
 int smla_select_cache_rows(const float *weights, int64_t weights_stride, int width, const int32_t *cache_seqlens,
                            int batch, int budget, int recent, int32_t *rows, int32_t *kept, float *kept_weights,
                            void *stream) {

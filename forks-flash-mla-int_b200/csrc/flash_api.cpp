@@ -539,6 +539,14 @@ Tensor mla_cache_row_weights(const Tensor &q_in, const Tensor &cache, const Tens
     p.weights_width = static_cast<int32_t>(weights.size(1));
     p.weights_stride = row_stride_2d(weights);
     p.accumulate = given ? 1 : 0;
+    std::optional<Tensor> workspace;             // freed stream-ordered by torch's allocator
+    if (SQ * H > 128) {
+        check_rc(smla_cache_row_weights_workspace(p.seqlen_q, p.num_heads, &p.workspace_bytes), what);
+        if (p.workspace_bytes > 0) {
+            workspace = empty_on(device, {static_cast<int64_t>((p.workspace_bytes + 3) / 4)}, aoti_torch_dtype_float32());
+            p.workspace = workspace->data_ptr();
+        }
+    }
     check_rc(smla_cache_row_weights(&p, current_stream(device)), what);
     return weights;
 }

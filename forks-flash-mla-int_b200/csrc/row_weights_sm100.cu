@@ -42,12 +42,23 @@ struct WeightsArgs {
     int width, accumulate, batch, s_q, heads, columns, causal, k_slabs;
     int num_blocks, page, box_rows, max_blocks;
     float scale_log2;
+    // RES with scratch: the blocks of columns of all tiles are dealt out, and a tile that is cut leaves its sums here, 2 slots
+    // of 128 per CTA (the end of a tile begun by a CTA before, the begin of one ended by a CTA behind), each with {sequence,
+    // first row, first block, end block}
+    float *part;
+    int4 *desc;
     int *status;
 };
 
 // RES: the rows stay while the columns pass.  N: columns of a score block.
+// A score is a sum over nine (eight) slabs of 64 dims.  The tensor pipe cuts off what an addition leaves below the
+// accumulator's last bit, which over 36 additions to a sum of size 200 makes 5e-6 of a weight.  Where tensor memory has
+// room the slabs go to several accumulators that are added up with proper rounding: each is smaller and takes fewer
+// additions (one sequence, 16 columns: 4.5e-6 -> see kGroups).
 template <bool RES, int N>
 struct Smem {
+    static constexpr int kPerGroup = RES ? 9 : N == 16 ? 1 : N == 32 ? 2 : N == 64 ? 3 : 5;      // slabs of an accumulator
+    static constexpr int kGroups = (9 + kPerGroup - 1) / kPerGroup;
     static constexpr int kQSlab = N * 128;
     static constexpr int kStage = RES ? kQSlab : kSlab + kQSlab;
     static constexpr int kStages = RES ? 2 : (208 * 1024 / kStage < 12 ? 208 * 1024 / kStage : 12);
@@ -59,10 +70,11 @@ struct Smem {
     static constexpr int kBarFull = 0, kBarEmpty = kStages, kBarKFull = 2 * kStages, kBarKEmpty = kBarKFull + kResident,
                          kBarS = kBarKEmpty + kResident, kBarSFree = kBarS + 2, kBarRecFull = kBarSFree + 2,
                          kBarRecEmpty = kBarRecFull + kRecords, kNumBars = kBarRecEmpty + kRecords;
-    static constexpr int kRecs = kBars + kNumBars * 8;                   // {valid, sequence, first row, length}
-    static constexpr int kMisc = kRecs + kRecords * 16;
+    static constexpr int kRecs = kBars + kNumBars * 8;                   // {valid, sequence, first row, length, first block, end block}
+    static constexpr int kMisc = kRecs + kRecords * 32;
     static constexpr int kBytes = kMisc + 16;
-    static constexpr int kTmemCols = 2 * N < 32 ? 32 : 2 * N;
+    static constexpr int kTmemCols = 512;
+    static_assert(2 * N * kGroups <= kTmemCols, "two score blocks in tensor memory");
 };
 static_assert(Smem<true, 256>::kBytes <= 232448 && Smem<false, 128>::kBytes <= 232448, "shared memory of one CTA");
 
@@ -84,19 +96,26 @@ template <bool RES, int N>
 __device__ __forceinline__ void loader_role(const WeightsArgs &a, uint8_t *smem, volatile int *abort_flag, int lane) {
     using L = Smem<RES, N>;
     const uint32_t bars = smem_u32(smem + L::kBars), ring = smem_u32(smem + L::kRingAt), ks = smem_u32(smem);
-    // this CTA's range of the tiles of all sequences
+    // This CTA's range of the tiles of all sequences, or of their blocks of columns.
+    const int blocks = RES ? (a.columns + N - 1) / N : 1, per_tile = RES && a.part != nullptr ? blocks : 1;
     long long total = 0;
     for (int b0 = 0; b0 < a.batch; b0 += 32)
         total += __reduce_add_sync(0xffffffffu, b0 + lane < a.batch ? (rows_of(a, b0 + lane) + 127) >> 7 : 0);
-    const long long first = total * blockIdx.x / gridDim.x, end = total * (blockIdx.x + 1) / gridDim.x;
-    const int boxes = 128 / a.box_rows, blocks = RES ? (a.columns + N - 1) / N : 1;
+    total *= per_tile;
+    const long long end = total * (blockIdx.x + 1) / gridDim.x;
+    const int boxes = 128 / a.box_rows;
+    if (RES && a.part != nullptr && lane < 2) a.desc[2 * blockIdx.x + lane] = make_int4(-1, 0, 0, 0);
+    __syncwarp();
     long long base = 0;                          // tiles in front of the 32 sequences at b0
     int b0 = 0, rec_i = 0;
     uint32_t st = 0, tile_n = 0, k_loads = 0;
     bool ok = true;
-    for (long long idx = first; ok; ++idx, ++rec_i) {
+    for (long long at_unit = total * blockIdx.x / gridDim.x; ok; ++rec_i) {
         int b = -1, t = 0;
-        while (idx < end && b0 < a.batch) {
+        const long long idx = at_unit / per_tile;
+        const int cb0 = static_cast<int>(at_unit - idx * per_tile);
+        const int cb1 = per_tile == 1 ? blocks : static_cast<int>(min(static_cast<long long>(blocks), end - idx * per_tile));
+        while (at_unit < end && b0 < a.batch) {
             const int n = b0 + lane < a.batch ? (rows_of(a, b0 + lane) + 127) >> 7 : 0;
             int upto = n;
 #pragma unroll
@@ -115,16 +134,19 @@ __device__ __forceinline__ void loader_role(const WeightsArgs &a, uint8_t *smem,
             base += __shfl_sync(0xffffffffu, upto, 31);
             b0 += 32;
         }
+        at_unit = (idx + 1) * per_tile;
         const int slot = rec_i % kRecords;
         if (!(ok = mbar_wait(bars + (L::kBarRecEmpty + slot) * 8, ((rec_i / kRecords) & 1) ^ 1, abort_flag))) break;
         if (lane == 0) {
-            int *rec = reinterpret_cast<int *>(smem + L::kRecs) + slot * 4;
+            int *rec = reinterpret_cast<int *>(smem + L::kRecs) + slot * 8;
             int len = 0;
             if (b >= 0) rows_of(a, b, &len);
             rec[0] = b >= 0;
             rec[1] = b;
             rec[2] = t * 128;
             rec[3] = len;
+            rec[4] = cb0;
+            rec[5] = cb1;
             mbar_arrive(bars + (L::kBarRecFull + slot) * 8);
         }
         __syncwarp();
@@ -138,9 +160,9 @@ __device__ __forceinline__ void loader_role(const WeightsArgs &a, uint8_t *smem,
             if (page < 0 || page > a.num_blocks) page = a.num_blocks;
         }
         const int q_row = b * a.columns;
-        for (int cb = 0; cb < blocks && ok; ++cb) {
+        for (int cb = cb0; cb < cb1 && ok; ++cb) {
             for (int s = 0; s < a.k_slabs; ++s, ++st) {
-                if (RES && cb == 0) {
+                if (RES && cb == cb0) {
                     if (!(ok = mbar_wait(bars + (L::kBarKEmpty + s) * 8, (tile_n & 1) ^ 1, abort_flag))) break;
                     if (lane == 0) mbar_arrive_expect_tx(bars + (L::kBarKFull + s) * 8, kSlab);
                     __syncwarp();
@@ -183,30 +205,31 @@ __device__ __forceinline__ void mma_role(const WeightsArgs &a, uint8_t *smem, ui
     const uint32_t go = elect_one();
     constexpr uint32_t idesc = umma_idesc_bf16(128, N, 0, 0);
     const uint64_t kd = umma_desc_sw128(RES ? smem_u32(smem) : ring, 16), qd = umma_desc_sw128(ring + (RES ? 0 : kSlab), 16);
-    const int blocks = RES ? (a.columns + N - 1) / N : 1;
     uint32_t st = 0, n_blocks = 0;
     bool ok = true;
     for (int it = 0; ok; ++it) {
         const int slot = it % kRecords;
         if (!(ok = mbar_wait(bars + (L::kBarRecFull + slot) * 8, (it / kRecords) & 1, abort_flag))) break;
-        const int valid = reinterpret_cast<const volatile int *>(smem + L::kRecs)[slot * 4];
+        const volatile int *rec = reinterpret_cast<const int *>(smem + L::kRecs) + slot * 8;
+        const int valid = rec[0], cb0 = rec[4], cb1 = rec[5];
         __syncwarp();
         if (lane == 0) mbar_arrive(bars + (L::kBarRecEmpty + slot) * 8);
         if (!valid) break;
-        for (int cb = 0; cb < blocks && ok; ++cb, ++n_blocks) {
+        for (int cb = cb0; cb < cb1 && ok; ++cb, ++n_blocks) {
             const int buf = n_blocks & 1;
             if (!(ok = mbar_wait(bars + (L::kBarSFree + buf) * 8, ((n_blocks >> 1) & 1) ^ 1, abort_flag))) break;
             for (int s = 0; s < a.k_slabs; ++s, ++st) {
-                if (RES && cb == 0 && !(ok = mbar_wait(bars + (L::kBarKFull + s) * 8, it & 1, abort_flag))) break;
+                if (RES && cb == cb0 && !(ok = mbar_wait(bars + (L::kBarKFull + s) * 8, it & 1, abort_flag))) break;
                 const uint32_t at = st % L::kStages;
                 if (!(ok = mbar_wait(bars + (L::kBarFull + at) * 8, (st / L::kStages) & 1, abort_flag))) break;
                 tc_fence_after_sync();
                 const uint64_t ka = kd + static_cast<uint64_t>((RES ? s * kSlab : at * L::kStage) >> 4);
                 const uint64_t qb = qd + static_cast<uint64_t>((at * L::kStage) >> 4);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) umma_bf16_ss_pred(tmem + buf * N, ka + 2 * k, qb + 2 * k, idesc, (s | k) != 0 ? 1u : 0u, go);
+                for (int k = 0; k < 4; ++k)
+                    umma_bf16_ss_pred(tmem + (buf * L::kGroups + s / L::kPerGroup) * N, ka + 2 * k, qb + 2 * k, idesc, s % L::kPerGroup || k ? 1u : 0u, go);
                 umma_commit_pred(bars + (L::kBarEmpty + at) * 8, go);
-                if (RES && cb + 1 == blocks) umma_commit_pred(bars + (L::kBarKEmpty + s) * 8, go);
+                if (RES && cb + 1 == cb1) umma_commit_pred(bars + (L::kBarKEmpty + s) * 8, go);
             }
             if (ok) umma_commit_pred(bars + (L::kBarS + buf) * 8, go);
         }
@@ -215,15 +238,28 @@ __device__ __forceinline__ void mma_role(const WeightsArgs &a, uint8_t *smem, ui
 }
 
 // ------------------------------------------------------------------ sums
-// Sum of exp2(s c - lse2) over `kCols` columns of this lane; with MASK only the columns in [lo, hi).
-template <int kCols, bool MASK>
-__device__ __forceinline__ void add_columns(uint32_t taddr, const float *lse2, float c, int lo, int hi, uint64_t (&acc)[4]) {
+// Sum of exp2(s c - lse2) over `kCols` columns of this lane, each the sum of `groups` accumulators N columns apart; with MASK
+// only the columns in [lo, hi).
+template <int kCols, int N, int kGroups, bool MASK>
+__device__ __forceinline__ void add_columns(uint32_t taddr, int groups, const float *lse2, float c, int lo, int hi, uint64_t (&acc)[4]) {
     uint32_t s[kCols];
-    if constexpr (kCols == 32) {
-        tmem_ld_x32_nowait(taddr, s);
-        tmem_ld_wait();
-    } else {
-        tmem_ld_x16(taddr, s);
+    const auto load = [](uint32_t at, uint32_t (&r)[kCols]) {
+        if constexpr (kCols == 32) {
+            tmem_ld_x32_nowait(at, r);
+            tmem_ld_wait();
+        } else {
+            tmem_ld_x16(at, r);
+        }
+    };
+    load(taddr, s);
+    if constexpr (kGroups > 1) {
+#pragma unroll 1
+        for (int g = 1; g < groups; ++g) {
+            uint32_t x[kCols];
+            load(taddr + g * N, x);
+#pragma unroll
+            for (int j = 0; j < kCols; ++j) s[j] = __float_as_uint(__uint_as_float(s[j]) + __uint_as_float(x[j]));
+        }
     }
     const uint64_t c2 = pack2(c, c);
 #pragma unroll
@@ -250,8 +286,8 @@ __device__ __forceinline__ void sum_role(const WeightsArgs &a, uint8_t *smem, ui
     const int group = warp >> 2, lane_row = (warp & 3) * 32 + lane;
     float *lse2 = reinterpret_cast<float *>(smem + L::kLse) + group * N;
     float *sums = reinterpret_cast<float *>(smem + L::kSums);
-    const uint32_t t_addr = tmem + group * N + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-    const int blocks = RES ? (a.columns + N - 1) / N : 1;
+    const uint32_t t_addr = tmem + group * N * L::kGroups + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    const int blocks = RES ? (a.columns + N - 1) / N : 1, groups = (a.k_slabs + L::kPerGroup - 1) / L::kPerGroup;
     uint32_t n_blocks = 0;
     bool failed = false;
     for (int it = 0;; ++it) {
@@ -262,8 +298,8 @@ __device__ __forceinline__ void sum_role(const WeightsArgs &a, uint8_t *smem, ui
             if (lane == 0) give_up(abort_flag, a.status, kStatusSoftmaxWait);
             return;
         }
-        const volatile int *rec = reinterpret_cast<const int *>(smem + L::kRecs) + slot * 4;
-        const int valid = rec[0], b = rec[1], row = rec[2] + lane_row, len = rec[3];
+        const volatile int *rec = reinterpret_cast<const int *>(smem + L::kRecs) + slot * 8;
+        const int valid = rec[0], b = rec[1], rec_row = rec[2], row = rec_row + lane_row, len = rec[3], cb0 = rec[4], cb1 = rec[5];
         __syncwarp();
         if (lane == 0) mbar_arrive(bars + (L::kBarRecEmpty + slot) * 8);
         if (!valid) return;
@@ -271,7 +307,7 @@ __device__ __forceinline__ void sum_role(const WeightsArgs &a, uint8_t *smem, ui
         const int from = a.causal ? max(0, row - len + a.s_q) * a.heads : 0;
         const int from_warp = a.causal ? max(0, row - lane + 31 - len + a.s_q) * a.heads : 0;
         float total = 0.0f, lost = 0.0f;         // compensated sum over the blocks
-        for (int cb = 0; cb < blocks; ++cb, ++n_blocks) {
+        for (int cb = cb0; cb < cb1; ++cb, ++n_blocks) {
             if ((n_blocks & 1) != static_cast<uint32_t>(group)) continue;
             const int c0 = cb * N;
             for (int x = lane_row; x < N; x += 128) {
@@ -289,11 +325,11 @@ __device__ __forceinline__ void sum_role(const WeightsArgs &a, uint8_t *smem, ui
             uint64_t acc[4] = {0, 0, 0, 0};
             if (from_warp <= c0 && c0 + N <= a.columns) {
 #pragma unroll 2
-                for (int j = 0; j < N; j += kCols) add_columns<kCols, false>(t_addr + j, lse2 + j, a.scale_log2, 0, 0, acc);
+                for (int j = 0; j < N; j += kCols) add_columns<kCols, N, L::kGroups, false>(t_addr + j, groups, lse2 + j, a.scale_log2, 0, 0, acc);
             } else {
                 // columns of the block that count for this row (those past the last hold other queries' scores)
                 const int lo = from - c0, hi = a.columns - c0;
-                for (int j = 0; j < N; j += kCols) add_columns<kCols, true>(t_addr + j, lse2 + j, a.scale_log2, lo - j, hi - j, acc);
+                for (int j = 0; j < N; j += kCols) add_columns<kCols, N, L::kGroups, true>(t_addr + j, groups, lse2 + j, a.scale_log2, lo - j, hi - j, acc);
             }
             tc_fence_before_sync();
             named_bar_sync(1 + group, 128);      // the scores and the lse buffer have been read
@@ -312,7 +348,13 @@ __device__ __forceinline__ void sum_role(const WeightsArgs &a, uint8_t *smem, ui
             named_bar_sync(3, 256);
             if (group == 0) {
                 total += sums[lane_row];
-                if (mine) *dst = a.accumulate ? *dst + total : total;
+                if (cb0 == 0 && cb1 == blocks) {
+                    if (mine) *dst = a.accumulate ? *dst + total : total;
+                } else {
+                    const int place = 2 * blockIdx.x + (cb0 == 0 ? 1 : 0);
+                    a.part[place * 128 + lane_row] = total;
+                    if (lane_row == 0) a.desc[place] = make_int4(b, rec_row, cb0, cb1);
+                }
             }
             named_bar_sync(3, 256);
         } else if (((n_blocks - 1) & 1) == static_cast<uint32_t>(group) && mine) {
@@ -380,6 +422,25 @@ __global__ void __launch_bounds__(kThreads, 1) row_weights_kernel(const __grid_c
     }
 }
 
+// The tiles that were cut: the block of the CTA that has a tile's first columns adds up its pieces, in the order of the CTAs.
+__global__ void __launch_bounds__(128) row_weights_join_kernel(const WeightsArgs a, int blocks, int ctas) {
+    const int4 d = a.desc[2 * blockIdx.x + 1];
+    if (d.x < 0) return;
+    float total = a.part[(2 * blockIdx.x + 1) * 128 + threadIdx.x];
+    int end = d.w;
+    for (int c = blockIdx.x + 1; end < blocks && c < ctas; ++c) {
+        const int4 e = a.desc[2 * c];
+        if (e.x < 0) continue;                   // a CTA without a share
+        if (e.x != d.x || e.y != d.y || e.z != end) break;
+        total += a.part[2 * c * 128 + threadIdx.x];
+        end = e.w;
+    }
+    const int row = d.y + threadIdx.x;
+    if (row >= rows_of(a, d.x)) return;
+    float *dst = a.weights + d.x * a.w_stride + row;
+    *dst = a.accumulate ? *dst + total : total;
+}
+
 template <bool RES, int N>
 int launch(WeightsArgs &a, unsigned grid, cudaStream_t stream) {
     static KernelSetup setup;
@@ -390,6 +451,10 @@ int launch(WeightsArgs &a, unsigned grid, cudaStream_t stream) {
 }
 
 }  // namespace
+
+size_t row_weights_workspace(int seqlen_q, int num_heads, int sm_count) {
+    return static_cast<int64_t>(seqlen_q) * num_heads <= 128 ? 0 : static_cast<size_t>(sm_count) * 2 * (128 * sizeof(float) + sizeof(int4));
+}
 
 int launch_row_weights(const smla_row_weights_params_t &p, int sm_count, cudaStream_t stream) {
     WeightsArgs a = {};
@@ -421,12 +486,27 @@ int launch_row_weights(const smla_row_weights_params_t &p, int sm_count, cudaStr
     a.scale_log2 = p.softmax_scale * kLog2e;
     const int64_t rows = std::min<int64_t>(p.weights_width, static_cast<int64_t>(p.max_blocks_per_seq) * p.page_block_size);
     const int64_t tiles = std::max<int64_t>(1, (rows + 127) / 128) * p.batch;
+    if (a.columns > 128) {
+        // With scratch every SM gets a share, down to a block of columns; else whole tiles are dealt out.
+        const int blocks = (a.columns + 255) / 256;
+        int64_t grid = std::min<int64_t>(tiles, sm_count);
+        const bool split = p.workspace != nullptr && p.workspace_bytes >= row_weights_workspace(p.seqlen_q, p.num_heads, sm_count);
+        if (split) {
+            if (reinterpret_cast<uintptr_t>(p.workspace) & 15u) return SMLA_EALIGN;
+            grid = std::min<int64_t>(tiles * blocks, sm_count);
+            a.desc = static_cast<int4 *>(p.workspace);
+            a.part = reinterpret_cast<float *>(a.desc + 2 * grid);
+        }
+        const int rc = launch<true, 256>(a, static_cast<unsigned>(grid), stream);
+        if (rc != 0 || !split) return rc;
+        row_weights_join_kernel<<<static_cast<unsigned>(grid), 128, 0, stream>>>(a, blocks, static_cast<int>(grid));
+        return static_cast<int>(cudaGetLastError());
+    }
     const unsigned grid = static_cast<unsigned>(std::min<int64_t>(tiles, sm_count));
     if (a.columns <= 16) return launch<false, 16>(a, grid, stream);
     if (a.columns <= 32) return launch<false, 32>(a, grid, stream);
     if (a.columns <= 64) return launch<false, 64>(a, grid, stream);
-    if (a.columns <= 128) return launch<false, 128>(a, grid, stream);
-    return launch<true, 256>(a, grid, stream);
+    return launch<false, 128>(a, grid, stream);
 }
 
 }  // namespace smla

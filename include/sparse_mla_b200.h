@@ -253,7 +253,14 @@ typedef struct smla_row_weights_params {
     int64_t weights_stride;               /* elements between sequences                                          */
     int32_t weights_width;                /* rows past it are left out                                           */
     int32_t accumulate;
+    void *workspace;                      /* 16-byte aligned scratch of smla_cache_row_weights_workspace bytes, which lets
+                                             windows of more than 128 (position, head) pairs use every SM; NULL or less:
+                                             whole tiles of 128 rows are dealt out.  Calls that overlap on the GPU need
+                                             one each                                                             */
+    size_t workspace_bytes;
 } smla_row_weights_params_t;
+/* Scratch for smla_cache_row_weights on the current device (0 where it needs none). */
+SMLA_API int smla_cache_row_weights_workspace(int seqlen_q, int num_heads, size_t *bytes);
 SMLA_API int smla_cache_row_weights(const smla_row_weights_params_t *params, void *stream);
 
 /* 2. smla_select_cache_rows: the rows of each sequence that stay when at most `budget` may.  All of them when the
