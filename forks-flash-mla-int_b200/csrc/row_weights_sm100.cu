@@ -59,9 +59,9 @@ template <bool RES, int N>
 struct Smem {
     static constexpr int kPerGroup = RES ? 9 : N == 16 ? 1 : N == 32 ? 2 : N == 64 ? 3 : 5;      // slabs of an accumulator
     static constexpr int kGroups = (9 + kPerGroup - 1) / kPerGroup;
-    static constexpr int kQSlab = N * 128;
+    static constexpr int kQSlab = (RES ? N / 2 : N) * 128;               // a CTA of a pair has half of the columns
     static constexpr int kStage = RES ? kQSlab : kSlab + kQSlab;
-    static constexpr int kStages = RES ? 2 : (208 * 1024 / kStage < 12 ? 208 * 1024 / kStage : 12);
+    static constexpr int kStages = RES ? 4 : (208 * 1024 / kStage < 12 ? 208 * 1024 / kStage : 12);
     static constexpr int kResident = RES ? 9 : 0;
     static constexpr int kRingAt = kResident * kSlab;
     static constexpr int kLse = kRingAt + kStages * kStage;              // two buffers of N floats
@@ -96,13 +96,16 @@ template <bool RES, int N>
 __device__ __forceinline__ void loader_role(const WeightsArgs &a, uint8_t *smem, volatile int *abort_flag, int lane) {
     using L = Smem<RES, N>;
     const uint32_t bars = smem_u32(smem + L::kBars), ring = smem_u32(smem + L::kRingAt), ks = smem_u32(smem);
-    // This CTA's range of the tiles of all sequences, or of their blocks of columns.
+    // This CTA's (pair's) range of the tiles of all sequences, or of their blocks of columns.
+    constexpr int kRows = RES ? 256 : 128;       // rows of a tile: 128 in each CTA
     const int blocks = RES ? (a.columns + N - 1) / N : 1, per_tile = RES && a.part != nullptr ? blocks : 1;
     long long total = 0;
     for (int b0 = 0; b0 < a.batch; b0 += 32)
-        total += __reduce_add_sync(0xffffffffu, b0 + lane < a.batch ? (rows_of(a, b0 + lane) + 127) >> 7 : 0);
+        total += __reduce_add_sync(0xffffffffu, b0 + lane < a.batch ? (rows_of(a, b0 + lane) + kRows - 1) / kRows : 0);
     total *= per_tile;
-    const long long end = total * (blockIdx.x + 1) / gridDim.x;
+    const unsigned team = RES ? blockIdx.x >> 1 : blockIdx.x, teams = RES ? gridDim.x >> 1 : gridDim.x;
+    const int rank = RES ? static_cast<int>(cluster_rank()) : 0;
+    const long long end = total * (team + 1) / teams;
     const int boxes = 128 / a.box_rows;
     if (RES && a.part != nullptr && lane < 2) a.desc[2 * blockIdx.x + lane] = make_int4(-1, 0, 0, 0);
     __syncwarp();
@@ -110,13 +113,13 @@ __device__ __forceinline__ void loader_role(const WeightsArgs &a, uint8_t *smem,
     int b0 = 0, rec_i = 0;
     uint32_t st = 0, tile_n = 0, k_loads = 0;
     bool ok = true;
-    for (long long at_unit = total * blockIdx.x / gridDim.x; ok; ++rec_i) {
+    for (long long at_unit = total * team / teams; ok; ++rec_i) {
         int b = -1, t = 0;
         const long long idx = at_unit / per_tile;
         const int cb0 = static_cast<int>(at_unit - idx * per_tile);
         const int cb1 = per_tile == 1 ? blocks : static_cast<int>(min(static_cast<long long>(blocks), end - idx * per_tile));
         while (at_unit < end && b0 < a.batch) {
-            const int n = b0 + lane < a.batch ? (rows_of(a, b0 + lane) + 127) >> 7 : 0;
+            const int n = b0 + lane < a.batch ? (rows_of(a, b0 + lane) + kRows - 1) / kRows : 0;
             int upto = n;
 #pragma unroll
             for (int d = 1; d < 32; d <<= 1) {
@@ -143,7 +146,7 @@ __device__ __forceinline__ void loader_role(const WeightsArgs &a, uint8_t *smem,
             if (b >= 0) rows_of(a, b, &len);
             rec[0] = b >= 0;
             rec[1] = b;
-            rec[2] = t * 128;
+            rec[2] = t * kRows + rank * 128;
             rec[3] = len;
             rec[4] = cb0;
             rec[5] = cb1;
@@ -154,7 +157,7 @@ __device__ __forceinline__ void loader_role(const WeightsArgs &a, uint8_t *smem,
         // the pages of the tile's boxes; one outside the table or the cache lies past the tensor's end: zeros
         int page = a.num_blocks, in_page = 0;
         if (lane < boxes) {
-            const int row = t * 128 + lane * a.box_rows, col = row / a.page;
+            const int row = t * kRows + rank * 128 + lane * a.box_rows, col = row / a.page;
             in_page = row - col * a.page;
             if (col < a.max_blocks) page = __ldg(a.table + b * a.table_stride + col);
             if (page < 0 || page > a.num_blocks) page = a.num_blocks;
@@ -164,36 +167,45 @@ __device__ __forceinline__ void loader_role(const WeightsArgs &a, uint8_t *smem,
             for (int s = 0; s < a.k_slabs; ++s, ++st) {
                 if (RES && cb == cb0) {
                     if (!(ok = mbar_wait(bars + (L::kBarKEmpty + s) * 8, (tile_n & 1) ^ 1, abort_flag))) break;
-                    if (lane == 0) mbar_arrive_expect_tx(bars + (L::kBarKFull + s) * 8, kSlab);
+                    const uint32_t full = bars + (L::kBarKFull + s) * 8;
+                    if (lane == 0 && rank == 0) mbar_arrive_expect_tx(full, 2 * kSlab);
                     __syncwarp();
                     if (lane < boxes)
-                        tma_load_3d(ks + s * kSlab + lane * a.box_rows * 128, &a.k_map, bars + (L::kBarKFull + s) * 8, s * 64, in_page, page);
+                        tma_load_3d_pair(ks + s * kSlab + lane * a.box_rows * 128, &a.k_map, map_rank(full, 0), s * 64, in_page, page);
                     ++k_loads;
                 }
                 const uint32_t at = st % L::kStages, full = bars + (L::kBarFull + at) * 8, dst = ring + at * L::kStage;
                 if (!(ok = mbar_wait(bars + (L::kBarEmpty + at) * 8, ((st / L::kStages) & 1) ^ 1, abort_flag))) break;
-                if (lane == 0) {
-                    mbar_arrive_expect_tx(full, L::kStage);
-                    constexpr int kBox = N < 128 ? N : 128;
-#pragma unroll
-                    for (int x = 0; x < N / kBox; ++x)
-                        tma_load_3d(dst + (RES ? 0 : kSlab) + x * kBox * 128, &a.q_map, full, s * 64, q_row + cb * N + x * kBox, 0);
+                if constexpr (RES) {
+                    if (lane == 0) {
+                        if (rank == 0) mbar_arrive_expect_tx(full, 2 * L::kStage);
+                        tma_load_3d_pair(dst, &a.q_map, map_rank(full, 0), s * 64, q_row + cb * N + rank * (N / 2), 0);
+                    }
+                    __syncwarp();
+                } else {
+                    if (lane == 0) {
+                        mbar_arrive_expect_tx(full, L::kStage);
+                        tma_load_3d(dst + kSlab, &a.q_map, full, s * 64, q_row, 0);
+                    }
+                    __syncwarp();
+                    if (lane < boxes) tma_load_3d(dst + lane * a.box_rows * 128, &a.k_map, full, s * 64, in_page, page);
                 }
-                __syncwarp();
-                if (!RES && lane < boxes) tma_load_3d(dst + lane * a.box_rows * 128, &a.k_map, full, s * 64, in_page, page);
             }
         }
         if (ok) ++tile_n;
     }
     if (!ok) {
-        // the copies in flight have to land before the CTA may end
+        // The copies in flight have to land before the CTA may end.  Those of a pair are counted on the even CTA's barriers,
+        // which wait for both CTAs' bytes; the odd one stays until the even one has seen them (cluster barrier at the end).
         if (lane == 0) give_up(abort_flag, a.status, kStatusGatherWait);
         __syncwarp();
         int never = 0;
-        for (uint32_t i = st > static_cast<uint32_t>(L::kStages) ? st - L::kStages : 0; i < st; ++i)
-            mbar_wait(bars + (L::kBarFull + i % L::kStages) * 8, (i / L::kStages) & 1, &never);
-        for (uint32_t i = k_loads > static_cast<uint32_t>(a.k_slabs) ? k_loads - a.k_slabs : 0; i < k_loads; ++i)
-            mbar_wait(bars + (L::kBarKFull + i % a.k_slabs) * 8, (i / a.k_slabs) & 1, &never);
+        if (rank == 0) {
+            for (uint32_t i = st > static_cast<uint32_t>(L::kStages) ? st - L::kStages : 0; i < st; ++i)
+                mbar_wait(bars + (L::kBarFull + i % L::kStages) * 8, (i / L::kStages) & 1, &never);
+            for (uint32_t i = k_loads > static_cast<uint32_t>(a.k_slabs) ? k_loads - a.k_slabs : 0; i < k_loads; ++i)
+                mbar_wait(bars + (L::kBarKFull + i % a.k_slabs) * 8, (i / a.k_slabs) & 1, &never);
+        }
     }
 }
 
@@ -203,7 +215,11 @@ __device__ __forceinline__ void mma_role(const WeightsArgs &a, uint8_t *smem, ui
     using L = Smem<RES, N>;
     const uint32_t bars = smem_u32(smem + L::kBars), ring = smem_u32(smem + L::kRingAt);
     const uint32_t go = elect_one();
-    constexpr uint32_t idesc = umma_idesc_bf16(128, N, 0, 0);
+    constexpr uint32_t idesc = umma_idesc_bf16(RES ? 256 : 128, N, 0, 0);
+    const auto commit = [&](uint32_t bar) {
+        if constexpr (RES) umma_commit_pair_pred(bar, go);
+        else umma_commit_pred(bar, go);
+    };
     const uint64_t kd = umma_desc_sw128(RES ? smem_u32(smem) : ring, 16), qd = umma_desc_sw128(ring + (RES ? 0 : kSlab), 16);
     uint32_t st = 0, n_blocks = 0;
     bool ok = true;
@@ -217,7 +233,8 @@ __device__ __forceinline__ void mma_role(const WeightsArgs &a, uint8_t *smem, ui
         if (!valid) break;
         for (int cb = cb0; cb < cb1 && ok; ++cb, ++n_blocks) {
             const int buf = n_blocks & 1;
-            if (!(ok = mbar_wait(bars + (L::kBarSFree + buf) * 8, ((n_blocks >> 1) & 1) ^ 1, abort_flag))) break;
+            const uint32_t s_free = bars + (L::kBarSFree + buf) * 8, s_phase = ((n_blocks >> 1) & 1) ^ 1;
+            if (!(ok = RES ? mbar_wait_cluster(s_free, s_phase, abort_flag) : mbar_wait(s_free, s_phase, abort_flag))) break;
             for (int s = 0; s < a.k_slabs; ++s, ++st) {
                 if (RES && cb == cb0 && !(ok = mbar_wait(bars + (L::kBarKFull + s) * 8, it & 1, abort_flag))) break;
                 const uint32_t at = st % L::kStages;
@@ -226,12 +243,15 @@ __device__ __forceinline__ void mma_role(const WeightsArgs &a, uint8_t *smem, ui
                 const uint64_t ka = kd + static_cast<uint64_t>((RES ? s * kSlab : at * L::kStage) >> 4);
                 const uint64_t qb = qd + static_cast<uint64_t>((at * L::kStage) >> 4);
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    umma_bf16_ss_pred(tmem + (buf * L::kGroups + s / L::kPerGroup) * N, ka + 2 * k, qb + 2 * k, idesc, s % L::kPerGroup || k ? 1u : 0u, go);
-                umma_commit_pred(bars + (L::kBarEmpty + at) * 8, go);
-                if (RES && cb + 1 == cb1) umma_commit_pred(bars + (L::kBarKEmpty + s) * 8, go);
+                for (int k = 0; k < 4; ++k) {
+                    const uint32_t d = tmem + (buf * L::kGroups + s / L::kPerGroup) * N, add = s % L::kPerGroup || k ? 1u : 0u;
+                    if constexpr (RES) umma_ss_pair_pred(d, ka + 2 * k, qb + 2 * k, idesc, add, go);
+                    else umma_bf16_ss_pred(d, ka + 2 * k, qb + 2 * k, idesc, add, go);
+                }
+                commit(bars + (L::kBarEmpty + at) * 8);
+                if (RES && cb + 1 == cb1) commit(bars + (L::kBarKEmpty + s) * 8);
             }
-            if (ok) umma_commit_pred(bars + (L::kBarS + buf) * 8, go);
+            if (ok) commit(bars + (L::kBarS + buf) * 8);
         }
     }
     if (!ok && lane == 0) give_up(abort_flag, a.status, kStatusMmaWait);
@@ -333,7 +353,11 @@ __device__ __forceinline__ void sum_role(const WeightsArgs &a, uint8_t *smem, ui
             }
             tc_fence_before_sync();
             named_bar_sync(1 + group, 128);      // the scores and the lse buffer have been read
-            if ((warp & 3) == 0 && lane == 0) mbar_arrive(bars + (L::kBarSFree + group) * 8);
+            if ((warp & 3) == 0 && lane == 0) {
+                const uint32_t s_free = bars + (L::kBarSFree + group) * 8;
+                if constexpr (RES) mbar_arrive_cluster(map_rank(s_free, 0));     // the even CTA issues for both
+                else mbar_arrive(s_free);
+            }
             const uint64_t both = add2(add2(acc[0], acc[1]), add2(acc[2], acc[3]));
             float x, y;
             unpack2(both, x, y);
@@ -374,6 +398,7 @@ __global__ void __launch_bounds__(kThreads, 1) row_weights_kernel(const __grid_c
         if (tid == 0) atomicOr(a.status, kStatusSmemLayout);
         return;
     }
+    const bool issues = !RES || cluster_rank() == 0;         // the products of a pair are issued by its even CTA
     if (tid == 0) {
         for (int i = 0; i < L::kStages; ++i) {
             mbar_init(bars + (L::kBarFull + i) * 8, 1);
@@ -385,24 +410,28 @@ __global__ void __launch_bounds__(kThreads, 1) row_weights_kernel(const __grid_c
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(bars + (L::kBarS + i) * 8, 1);
-            mbar_init(bars + (L::kBarSFree + i) * 8, 1);
+            mbar_init(bars + (L::kBarSFree + i) * 8, RES ? 2 : 1);
         }
         for (int i = 0; i < kRecords; ++i) {
             mbar_init(bars + (L::kBarRecFull + i) * 8, 1);
-            mbar_init(bars + (L::kBarRecEmpty + i) * 8, 9);
+            mbar_init(bars + (L::kBarRecEmpty + i) * 8, issues ? 9 : 8);
         }
         *abort_flag = 0;
         mbar_init_fence();
     }
-    if (warp == 8) tmem_alloc(smem_u32(smem + L::kMisc + 8), L::kTmemCols);
+    if (warp == 8) {
+        if constexpr (RES) tmem_alloc_pair(smem_u32(smem + L::kMisc + 8), L::kTmemCols);
+        else tmem_alloc(smem_u32(smem + L::kMisc + 8), L::kTmemCols);
+    }
     tc_fence_before_sync();
-    __syncthreads();
+    if constexpr (RES) cluster_sync_all();       // also: the other CTA's barriers are there
+    else __syncthreads();
     tc_fence_after_sync();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(smem + L::kMisc + 8);
     if (warp < 8) {
         sum_role<RES, N>(a, smem, tmem, abort_flag, warp, lane);
     } else if (warp == 8) {
-        mma_role<RES, N>(a, smem, tmem, abort_flag, lane);
+        if (issues) mma_role<RES, N>(a, smem, tmem, abort_flag, lane);
     } else if (warp == 9) {
         loader_role<RES, N>(a, smem, abort_flag, lane);
     } else if (!a.accumulate) {
@@ -415,10 +444,16 @@ __global__ void __launch_bounds__(kThreads, 1) row_weights_kernel(const __grid_c
         }
     }
     tc_fence_before_sync();
-    __syncthreads();
+    __syncwarp();
+    if constexpr (RES) cluster_sync_all();       // nothing of this CTA's is used by the other any more
+    else __syncthreads();
     if (warp == 8) {
-        tmem_relinquish();
-        tmem_dealloc(tmem, L::kTmemCols);
+        if constexpr (RES) {
+            tmem_free_pair(tmem, L::kTmemCols);
+        } else {
+            tmem_relinquish();
+            tmem_dealloc(tmem, L::kTmemCols);
+        }
     }
 }
 
@@ -428,7 +463,7 @@ __global__ void __launch_bounds__(128) row_weights_join_kernel(const WeightsArgs
     if (d.x < 0) return;
     float total = a.part[(2 * blockIdx.x + 1) * 128 + threadIdx.x];
     int end = d.w;
-    for (int c = blockIdx.x + 1; end < blocks && c < ctas; ++c) {
+    for (int c = blockIdx.x + 2; end < blocks && c < ctas; c += 2) {     // the same half of the next pair
         const int4 e = a.desc[2 * c];
         if (e.x < 0) continue;                   // a CTA without a share
         if (e.x != d.x || e.y != d.y || e.z != end) break;
@@ -446,8 +481,18 @@ int launch(WeightsArgs &a, unsigned grid, cudaStream_t stream) {
     static KernelSetup setup;
     const int rc = setup.get(reinterpret_cast<const void *>(&row_weights_kernel<RES, N>), Smem<RES, N>::kBytes, &a.status);
     if (rc != 0) return rc;
-    row_weights_kernel<RES, N><<<grid, kThreads, Smem<RES, N>::kBytes, stream>>>(a);
-    return static_cast<int>(cudaGetLastError());
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = Smem<RES, N>::kBytes;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = RES ? 2 : 1;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = RES ? 1 : 0;
+    return static_cast<int>(cudaLaunchKernelEx(&cfg, row_weights_kernel<RES, N>, a));
 }
 
 }  // namespace
@@ -489,11 +534,12 @@ int launch_row_weights(const smla_row_weights_params_t &p, int sm_count, cudaStr
     if (a.columns > 128) {
         // With scratch every SM gets a share, down to a block of columns; else whole tiles are dealt out.
         const int blocks = (a.columns + 255) / 256;
-        int64_t grid = std::min<int64_t>(tiles, sm_count);
+        const int64_t pair_tiles = std::max<int64_t>(1, (rows + 255) / 256) * p.batch;
+        int64_t grid = 2 * std::min<int64_t>(pair_tiles, sm_count / 2);
         const bool split = p.workspace != nullptr && p.workspace_bytes >= row_weights_workspace(p.seqlen_q, p.num_heads, sm_count);
         if (split) {
             if (reinterpret_cast<uintptr_t>(p.workspace) & 15u) return SMLA_EALIGN;
-            grid = std::min<int64_t>(tiles * blocks, sm_count);
+            grid = 2 * std::min<int64_t>(pair_tiles * blocks, sm_count / 2);
             a.desc = static_cast<int4 *>(p.workspace);
             a.part = reinterpret_cast<float *>(a.desc + 2 * grid);
         }
