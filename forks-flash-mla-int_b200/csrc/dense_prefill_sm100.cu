@@ -9,17 +9,24 @@
 // the first block of keys and hardly ever again.  Weights are rounded to the input type for the second product (the
 // tensor pipe multiplies 16-bit operands); the sum l takes them unrounded, in fp32.
 //
-// Work is cut into items: 256 query rows of one head, as two halves of 128 (the lanes of tensor memory).  A CTA
-// (persistent, one per SM) holds the item's Q (2 x 128 x d) in shared memory and walks the keys in blocks of 128:
-//   S_i = Q_i K^T  -> tensor memory, 128 columns of fp32 per half (both operands by descriptor from shared memory)
-//   P_i = exp(S_i - m)  -> 16-bit, written over S_i in tensor memory (64 columns)
-//   O_i += P_i V  -> tensor memory, 128 columns per half (P_i read from tensor memory, V from shared memory)
-// S0 | S1 | O0 | O1 take all 512 columns.  While one half's weights are computed the tensor pipe works on the other's.
-// K and V arrive by TMA as [128 rows][64 dims] slabs with the 128-byte swizzle in one ring; a slab read K-major gives
-// K for the first product and MN-major gives V for the second.
+// Work is cut into items: 256 query rows of one head, for a pair of CTAs (a cluster, persistent) that multiplies as one
+// with M = 256: each CTA has 128 of the rows, in the lanes of its tensor memory, and half of every key block.  The items'
+// key blocks of 128 form one sequence of tiles that runs on across items:
+//   S(g) = Q K(g)^T  -> one of three buffers of 128 columns in tensor memory
+//   P(g) = exp(S(g) - m)  -> 16-bit, written over S(g) (64 columns)
+//   O += P(g) V(g)  -> 128 columns
+// The products are issued in the order S(g + 2), O(g): the weights of a tile have the time of two tiles' products to be
+// computed in, and two warpgroups take turns at the tiles, so that a weight computation (about 2100 cycles for a tile, one
+// row per thread) may take nearly twice as long as the products of a tile (1280 cycles at 192 dims).  With one CTA per
+// item, S in one buffer for each half of the rows, the chain scores - weights - output - next scores bounded it: 1.05
+// PFLOP/s on a prompt of 16384 tokens.
+// K and V arrive by TMA as slabs of 64 dims with the 128-byte swizzle: of K the rows of 64 keys (its half of N), of V all
+// 128 keys of 64 of the dims (its half of N there).  A slab read K-major gives K for the first product, MN-major V for the
+// second.  Sharing B halves the fills: with both operands from shared memory one CTA's products alone (M = N = 128) take all
+// of its 128 bytes a cycle.
 //
-// Roles (384 threads): warps 0-3 and 4-7 are the softmax of the two halves (one row per thread), warp 8 issues the
-// MMAs, warp 9 finds the items and loads.  Item records go through a ring of four in shared memory.
+// Roles (384 threads): warps 0-3 and 4-7 are the two softmax warpgroups, warp 8 (of the even CTA) issues the products, warp 9
+// finds the items and loads Q and K, warp 10 loads V.  Item records go through a ring of four in shared memory.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -38,12 +45,14 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kThreads = 384;
 constexpr int kSlab = 128 * 128;                 // bytes of [128 rows][64 dims] of 16-bit elements
-constexpr int kSlabs = 14;                       // Q and ring together
+constexpr int kHalfSlab = kSlab / 2;             // [64 rows][64 dims]
 constexpr int kRecords = 4;
+constexpr int kRecInts = 12;
+constexpr int kBuffers = 3;                      // of S
+constexpr uint32_t kTmemO = kBuffers * 128;
 // Registers: 168 a thread at launch (the most that 384 threads can have); the softmax warps hold a row of 128 scores.
 constexpr int kRegsLaunch = 168, kRegsSoftmax = 208, kRegsOther = 88;
 static_assert(256 * kRegsSoftmax + 128 * kRegsOther <= kThreads * kRegsLaunch, "shares of the launch's registers");
-constexpr int kRecInts = 12;
 
 struct PrefillArgs {
     CUtensorMap q_map, k_map, v_map;
@@ -60,21 +69,27 @@ struct PrefillArgs {
 
 template <int DQK>
 struct Smem {
-    static constexpr int kDSlabs = DQK / 64;                 // slabs of a 128-row tile of Q or K
-    static constexpr int kRing = kSlabs - 2 * kDSlabs;       // 8 slabs at 192 dims, 10 at 128
-    static constexpr int kQ = 0;
-    static constexpr int kRingAt = 2 * kDSlabs * kSlab;
-    static constexpr int kBars = kSlabs * kSlab;
-    static constexpr int kBarFull = 0, kBarEmpty = kRing, kBarQFull = 2 * kRing, kBarQEmpty = kBarQFull + 1, kBarS = kBarQFull + 2,
-                         kBarP = kBarQFull + 4, kBarO = kBarQFull + 6, kBarRecFull = kBarQFull + 8, kBarRecEmpty = kBarRecFull + kRecords,
-                         kNumBars = kBarRecEmpty + kRecords;
+    static constexpr int kDSlabs = DQK / 64;
+    static constexpr int kQBytes = kDSlabs * kSlab, kKBytes = kDSlabs * kHalfSlab;     // of this CTA
+    static constexpr int kSlots = DQK == 192 ? 3 : 4;                    // K blocks, and V blocks, in flight
+    static constexpr int kQ = 0;                                         // two: the next item's is loaded early
+    static constexpr int kK = 2 * kQBytes;
+    static constexpr int kV = kK + kSlots * kKBytes;
+    static constexpr int kBars = kV + kSlots * kSlab;
+    static constexpr int kBarQFull = 0, kBarQEmpty = 2, kBarKFull = 4, kBarKEmpty = kBarKFull + kSlots, kBarVFull = kBarKEmpty + kSlots,
+                         kBarVEmpty = kBarVFull + kSlots, kBarS = kBarVEmpty + kSlots, kBarP = kBarS + kBuffers, kBarPv = kBarP + kBuffers,
+                         kBarO = kBarPv + 2, kBarRef = kBarO + 1, kBarTail = kBarRef + 8, kBarRecFull = kBarTail + 1,
+                         kBarRecEmpty = kBarRecFull + kRecords, kNumBars = kBarRecEmpty + kRecords;
     static constexpr int kRecs = kBars + kNumBars * 8;
-    static constexpr int kMisc = kRecs + kRecords * kRecInts * 4;        // abort flag, tensor memory address
+    static constexpr int kRef = kRecs + kRecords * kRecInts * 4;         // the rows' reference
+    static constexpr int kSums = kRef + 128 * 4;                         // {reference, sum} of each warpgroup at an item's end
+    static constexpr int kQueue = kSums + 2 * 128 * 8;                   // eight items {blocks, keys} with scores not yet added
+    static constexpr int kMisc = kQueue + 8 * 8;                         // abort flag, tensor memory address
     static constexpr int kBytes = kMisc + 16;
 };
 static_assert(Smem<192>::kBytes <= 232448 && Smem<128>::kBytes <= 232448, "shared memory of one CTA");
 
-enum { kRecValid, kRecQRow, kRecRows, kRecHead, kRecKRow, kRecNk, kRecOff, kRecN0, kRecN1 };
+enum { kRecValid, kRecQRow, kRecRows, kRecHead, kRecKRow, kRecNk, kRecOff, kRecN };
 
 __device__ __forceinline__ void give_up(volatile int *abort_flag, int *status, int bit) {
     *abort_flag = 1;
@@ -147,11 +162,7 @@ __device__ __forceinline__ bool find_item(const PrefillArgs &a, Walk &w, long lo
                 const int level = min(((w.bucket + 1) << w.shift) - 1, s.top) - (r - (before + upto - n));
                 const int m0 = (s.blocks - 1 - (s.top - level)) << 8;
                 const int rows = min(256, s.nq - m0), off = m0 + s.nk - s.nq;
-                int n0 = s.nk, n1 = s.nk;
-                if (a.causal) {
-                    n0 = min(s.nk, max(0, off + min(rows, 128)));
-                    n1 = min(s.nk, max(0, off + rows));
-                }
+                const int see = a.causal ? min(s.nk, max(0, off + rows)) : s.nk;         // keys that the item's last row sees
                 if (lane == src) {
                     rec[kRecValid] = 1;
                     rec[kRecQRow] = s.q0 + m0;
@@ -160,8 +171,7 @@ __device__ __forceinline__ bool find_item(const PrefillArgs &a, Walk &w, long lo
                     rec[kRecKRow] = s.k0;
                     rec[kRecNk] = s.nk;
                     rec[kRecOff] = off;
-                    rec[kRecN0] = (n0 + 127) >> 7;
-                    rec[kRecN1] = rows > 128 ? (n1 + 127) >> 7 : 0;
+                    rec[kRecN] = (see + 127) >> 7;
                 }
                 return true;
             }
@@ -172,167 +182,214 @@ __device__ __forceinline__ bool find_item(const PrefillArgs &a, Walk &w, long lo
     return false;
 }
 
-// ------------------------------------------------------------------ loader
+// ------------------------------------------------------------------ loaders
+// Records, Q and K.  Bytes of both CTAs are counted on the even one's barriers, whose products read them.
 template <int DQK>
-__device__ __forceinline__ void loader_role(const PrefillArgs &a, uint8_t *smem, volatile int *abort_flag, int lane) {
+__device__ __forceinline__ void qk_loader_role(const PrefillArgs &a, uint8_t *smem, volatile int *abort_flag, int rank, int lane) {
     using L = Smem<DQK>;
-    const uint32_t bars = smem_u32(smem + L::kBars), ring = smem_u32(smem + L::kRingAt), qs = smem_u32(smem + L::kQ);
+    const uint32_t bars = smem_u32(smem + L::kBars), qs = smem_u32(smem + L::kQ), ks = smem_u32(smem + L::kK);
+    const unsigned team = blockIdx.x >> 1, teams = gridDim.x >> 1;
     Walk w;
     start_walk(a, w, lane);
-    uint32_t slab = 0, nq_loads = 0;
+    uint32_t block = 0, nq = 0;
     bool ok = true;
     for (int it = 0; ok; ++it) {
         const int slot = it % kRecords;
         int *rec = reinterpret_cast<int *>(smem + L::kRecs) + slot * kRecInts;
         if (!(ok = mbar_wait(bars + (L::kBarRecEmpty + slot) * 8, ((it / kRecords) & 1) ^ 1, abort_flag))) break;
-        // back and forth over the CTAs: the one with the largest item of a round gets the smallest of the next
-        const unsigned turn = (it & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x;
-        const bool more = find_item(a, w, static_cast<long long>(it) * gridDim.x + turn, lane, rec);
+        // back and forth over the pairs: the one with the largest item of a round gets the smallest of the next
+        const unsigned turn = (it & 1) ? teams - 1 - team : team;
+        const bool more = find_item(a, w, static_cast<long long>(it) * teams + turn, lane, rec);
         if (!more && lane == 0) rec[kRecValid] = 0;
         __syncwarp();
         if (lane == 0) mbar_arrive(bars + (L::kBarRecFull + slot) * 8);
         if (!more) break;
         const volatile int *vr = rec;
-        const int n0 = vr[kRecN0], n1 = vr[kRecN1], n = max(n0, n1), head = vr[kRecHead], krow = vr[kRecKRow], qrow = vr[kRecQRow];
+        const int n = vr[kRecN], head = vr[kRecHead], krow = vr[kRecKRow] + rank * 64, qrow = vr[kRecQRow] + rank * 128;
         const int kv_head = head / a.group;
         if (n == 0) continue;
-        if (!(ok = mbar_wait(bars + L::kBarQEmpty * 8, (nq_loads & 1) ^ 1, abort_flag))) break;
-        ++nq_loads;
+        const uint32_t qb = nq & 1;
+        if (!(ok = mbar_wait(bars + (L::kBarQEmpty + qb) * 8, ((nq >> 1) & 1) ^ 1, abort_flag))) break;
+        ++nq;
         if (lane == 0) {
-            mbar_arrive_expect_tx(bars + L::kBarQFull * 8, ((n0 > 0) + (n1 > 0)) * L::kDSlabs * kSlab);
-            for (int i = 0; i < 2; ++i) {
-                if ((i ? n1 : n0) == 0) continue;
-                for (int s = 0; s < L::kDSlabs; ++s)
-                    tma_load_3d(qs + (i * L::kDSlabs + s) * kSlab, &a.q_map, bars + L::kBarQFull * 8, s * 64, qrow + i * 128, head);
-            }
+            const uint32_t full = bars + (L::kBarQFull + qb) * 8;
+            if (rank == 0) mbar_arrive_expect_tx(full, 2 * L::kQBytes);
+            for (int s = 0; s < L::kDSlabs; ++s)
+                tma_load_3d_pair(qs + qb * L::kQBytes + s * kSlab, &a.q_map, map_rank(full, 0), s * 64, qrow, head);
         }
-        for (int t = 0; t < n && ok; ++t) {
-            for (int s = 0; s < L::kDSlabs + 2; ++s, ++slab) {
-                const uint32_t at = slab % L::kRing;
-                if (!(ok = mbar_wait(bars + (L::kBarEmpty + at) * 8, ((slab / L::kRing) & 1) ^ 1, abort_flag))) break;
-                if (lane == 0) {
-                    mbar_arrive_expect_tx(bars + (L::kBarFull + at) * 8, kSlab);
-                    if (s < L::kDSlabs)
-                        tma_load_3d(ring + at * kSlab, &a.k_map, bars + (L::kBarFull + at) * 8, s * 64, krow + t * 128, kv_head);
-                    else
-                        tma_load_3d(ring + at * kSlab, &a.v_map, bars + (L::kBarFull + at) * 8, (s - L::kDSlabs) * 64, krow + t * 128, kv_head);
-                }
-                __syncwarp();
+        __syncwarp();
+        for (int t = 0; t < n; ++t, ++block) {
+            const uint32_t at = block % L::kSlots, full = bars + (L::kBarKFull + at) * 8;
+            if (!(ok = mbar_wait(bars + (L::kBarKEmpty + at) * 8, ((block / L::kSlots) & 1) ^ 1, abort_flag))) break;
+            if (lane == 0) {
+                if (rank == 0) mbar_arrive_expect_tx(full, 2 * L::kKBytes);
+                for (int s = 0; s < L::kDSlabs; ++s)
+                    tma_load_3d_pair(ks + at * L::kKBytes + s * kHalfSlab, &a.k_map, map_rank(full, 0), s * 64, krow + t * 128, kv_head);
             }
+            __syncwarp();
         }
     }
     if (!ok) {
-        // another role gave up, or this one: the copies in flight have to land before the CTA may end
+        // Another role gave up, or this one.  The copies in flight have to land before the CTA may end; the odd CTA's are
+        // counted by the even one, for which it waits at the end.
         if (lane == 0) give_up(abort_flag, a.status, kStatusGatherWait);
         __syncwarp();
         int never = 0;
-        const uint32_t first = slab > static_cast<uint32_t>(L::kRing) ? slab - L::kRing : 0;
-        for (uint32_t i = first; i < slab; ++i) mbar_wait(bars + (L::kBarFull + i % L::kRing) * 8, (i / L::kRing) & 1, &never);
-        if (nq_loads > 0) mbar_wait(bars + L::kBarQFull * 8, (nq_loads - 1) & 1, &never);
+        if (rank == 0) {
+            for (uint32_t i = block > static_cast<uint32_t>(L::kSlots) ? block - L::kSlots : 0; i < block; ++i)
+                mbar_wait(bars + (L::kBarKFull + i % L::kSlots) * 8, (i / L::kSlots) & 1, &never);
+            for (uint32_t i = nq > 2 ? nq - 2 : 0; i < nq; ++i) mbar_wait(bars + (L::kBarQFull + (i & 1)) * 8, (i >> 1) & 1, &never);
+        }
     }
 }
 
-// ------------------------------------------------------------------ MMA issue
-template <int DQK, bool FP16>
-__device__ __forceinline__ void mma_role(const PrefillArgs &a, uint8_t *smem, uint32_t tmem, volatile int *abort_flag, int lane) {
+template <int DQK>
+__device__ __forceinline__ void v_loader_role(const PrefillArgs &a, uint8_t *smem, volatile int *abort_flag, int rank, int lane) {
     using L = Smem<DQK>;
-    const uint32_t bars = smem_u32(smem + L::kBars), ring = smem_u32(smem + L::kRingAt);
-    const uint32_t go = elect_one();
-    constexpr uint32_t idesc_qk = umma_idesc_16(FP16, 128, 128, 0, 0);
-    constexpr uint32_t idesc_pv = umma_idesc_16(FP16, 128, 128, 0, 1);
-    constexpr uint32_t idesc_pv64 = umma_idesc_16(FP16, 128, 64, 0, 1);
-    const uint64_t qd = umma_desc_sw128(smem_u32(smem + L::kQ), 16), kd = umma_desc_sw128(ring, 16), vd = umma_desc_sw128(ring, kSlab);
-    constexpr int kPer = L::kDSlabs + 2;
-    uint32_t base = 0, nq_loads = 0, np[2] = {0, 0};
+    const uint32_t bars = smem_u32(smem + L::kBars), vs = smem_u32(smem + L::kV), tail = bars + L::kBarTail * 8;
+    uint32_t block = 0, tails = 0;
     bool ok = true;
-
     for (int it = 0; ok; ++it) {
         const int slot = it % kRecords;
         if (!(ok = mbar_wait(bars + (L::kBarRecFull + slot) * 8, (it / kRecords) & 1, abort_flag))) break;
         const volatile int *rec = reinterpret_cast<const int *>(smem + L::kRecs) + slot * kRecInts;
-        const int valid = rec[kRecValid], n0 = rec[kRecN0], n1 = rec[kRecN1], nk = rec[kRecNk];
+        const int valid = rec[kRecValid], n = rec[kRecN], nk = rec[kRecNk], krow = rec[kRecKRow], head = rec[kRecHead];
         __syncwarp();
         if (lane == 0) mbar_arrive(bars + (L::kBarRecEmpty + slot) * 8);
         if (!valid) break;
-        const int n = max(n0, n1);
-        if (n == 0) continue;
-        if (!(ok = mbar_wait(bars + L::kBarQFull * 8, nq_loads & 1, abort_flag))) break;
-        ++nq_loads;
-
-        // S_i = Q_i K(t)^T; the last user of the tile gives its slabs back, the last use of Q the Q tile
-        const auto qk = [&](int i, int t) {
-            const bool last = i == 1 || t >= n1;
-            for (int s = 0; s < L::kDSlabs; ++s) {
-                const uint32_t idx = base + t * kPer + s, at = idx % L::kRing;
-                if (!mbar_wait(bars + (L::kBarFull + at) * 8, (idx / L::kRing) & 1, abort_flag)) return false;
-                tc_fence_after_sync();
-                const uint64_t qa = qd + static_cast<uint64_t>(((i * L::kDSlabs + s) * kSlab) >> 4), kb = kd + static_cast<uint64_t>((at * kSlab) >> 4);
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    umma_bf16_ss_pred(tmem + i * 128, qa + 2 * k, kb + 2 * k, idesc_qk, (s | k) != 0 ? 1u : 0u, go);
-                if (last) umma_commit_pred(bars + (L::kBarEmpty + at) * 8, go);
-            }
-            umma_commit_pred(bars + (L::kBarS + i) * 8, go);
-            return true;
-        };
-        // O_i += P_i V(t)
-        const auto pv = [&](int i, int t) {
-            const bool first = i == 0 || t >= n0, last = i == 1 || t >= n1;
-            const uint32_t idx = base + t * kPer + L::kDSlabs;
-            const uint32_t at0 = idx % L::kRing, at1 = (idx + 1) % L::kRing;
-            if (!mbar_wait(bars + (L::kBarFull + at0) * 8, (idx / L::kRing) & 1, abort_flag)) return false;
-            if (!mbar_wait(bars + (L::kBarFull + at1) * 8, ((idx + 1) / L::kRing) & 1, abort_flag)) return false;
-            const int left = nk - t * 128, steps = left >= 128 ? 8 : (left + 15) >> 4;
-            if (first && left < 128 && (left & 15) != 0) {
-                // the last 16 rows that are multiplied reach past the sequence: what lies there (another sequence's
-                // rows, NaN) has weight 0, and 0 x NaN is NaN
-                const int r0 = left, r1 = (left + 15) & ~15;
-                for (int x = lane; x < (r1 - r0) * 16; x += 32) {
-                    const uint32_t dst = ring + ((x & 8) ? at1 : at0) * kSlab + (r0 + (x >> 4)) * 128 + (x & 7) * 16;
-                    asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(dst), "r"(0) : "memory");
+        const int kv_head = head / a.group;
+        for (int t = 0; t < n; ++t, ++block) {
+            const uint32_t at = block % L::kSlots, full = bars + (L::kBarVFull + at) * 8, dst = vs + at * kSlab;
+            if (!(ok = mbar_wait(bars + (L::kBarVEmpty + at) * 8, ((block / L::kSlots) & 1) ^ 1, abort_flag))) break;
+            const int left = nk - t * 128;
+            if (left >= 128 || (left & 15) == 0) {
+                if (lane == 0) {
+                    const uint32_t both = map_rank(full, 0);
+                    mbar_arrive_expect_tx_cluster(both, kSlab);
+                    tma_load_3d_pair(dst, &a.v_map, both, rank * 64, krow + t * 128, kv_head);
                 }
+                __syncwarp();
+            } else {
+                // The last 16 rows that are multiplied reach past the sequence: what lies there (another sequence's rows,
+                // NaN) has weight 0, and 0 x NaN is NaN.  They are cleared before the block is given to the products.
+                if (lane == 0) {
+                    mbar_arrive_expect_tx(tail, kSlab);
+                    tma_load_3d(dst, &a.v_map, tail, rank * 64, krow + t * 128, kv_head);
+                }
+                __syncwarp();
+                if (!(ok = mbar_wait(tail, tails++ & 1, abort_flag))) break;
+                const int r0 = left, r1 = (left + 15) & ~15;
+                for (int x = lane; x < (r1 - r0) * 8; x += 32)
+                    asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(dst + (r0 + (x >> 3)) * 128 + (x & 7) * 16), "r"(0) : "memory");
                 fence_async_smem();
                 __syncwarp();
-            }
-            tc_fence_after_sync();
-            const uint64_t v0 = vd + static_cast<uint64_t>((at0 * kSlab) >> 4), v1 = vd + static_cast<uint64_t>((at1 * kSlab) >> 4);
-            const uint32_t o = tmem + 256 + i * 128, p = tmem + i * 128;
-            if (at1 == at0 + 1) {
-                for (int k = 0; k < steps; ++k) umma_f16_ts_pred(o, p + k * 8, v0 + k * 128, idesc_pv, (t | k) != 0 ? 1u : 0u, go);
-            } else {                             // the pair lies at the two ends of the ring
-                for (int k = 0; k < steps; ++k) {
-                    umma_f16_ts_pred(o, p + k * 8, v0 + k * 128, idesc_pv64, (t | k) != 0 ? 1u : 0u, go);
-                    umma_f16_ts_pred(o + 64, p + k * 8, v1 + k * 128, idesc_pv64, (t | k) != 0 ? 1u : 0u, go);
-                }
-            }
-            if (last) {
-                umma_commit_pred(bars + (L::kBarEmpty + at0) * 8, go);
-                umma_commit_pred(bars + (L::kBarEmpty + at1) * 8, go);
-            }
-            return true;
-        };
-        for (int i = 0; i < 2 && ok; ++i)
-            if ((i ? n1 : n0) > 0) {
-                ok = qk(i, 0);
-                if (n == 1 && (i == 1 || n1 == 0)) umma_commit_pred(bars + L::kBarQEmpty * 8, go);
-            }
-        for (int t = 0; t < n && ok; ++t) {
-            for (int i = 0; i < 2 && ok; ++i) {
-                const int ni = i ? n1 : n0;
-                if (t >= ni) continue;
-                // the half's weights are in tensor memory (and its last item's output has been read)
-                if (!(ok = mbar_wait(bars + (L::kBarP + i) * 8, np[i] & 1, abort_flag))) break;
-                ++np[i];
-                if (!(ok = pv(i, t))) break;
-                if (t + 1 < ni) {
-                    if (!(ok = qk(i, t + 1))) break;
-                    if (t + 2 == n && (i == 1 || t + 1 >= n1)) umma_commit_pred(bars + L::kBarQEmpty * 8, go);
-                } else {
-                    umma_commit_pred(bars + (L::kBarO + i) * 8, go);
-                }
+                if (lane == 0) mbar_arrive_cluster(map_rank(full, 0));
             }
         }
-        base += n * kPer;
+    }
+    if (!ok) {
+        if (lane == 0) give_up(abort_flag, a.status, kStatusGatherWait);
+        __syncwarp();
+        int never = 0;
+        if (tails > 0) mbar_wait(tail, (tails - 1) & 1, &never);
+        if (rank == 0)
+            for (uint32_t i = block > static_cast<uint32_t>(L::kSlots) ? block - L::kSlots : 0; i < block; ++i)
+                mbar_wait(bars + (L::kBarVFull + i % L::kSlots) * 8, (i / L::kSlots) & 1, &never);
+    }
+}
+
+// ------------------------------------------------------------------ products (the even CTA, for both)
+template <int DQK, bool FP16>
+__device__ __forceinline__ void mma_role(const PrefillArgs &a, uint8_t *smem, uint32_t tmem, volatile int *abort_flag, int lane) {
+    using L = Smem<DQK>;
+    const uint32_t bars = smem_u32(smem + L::kBars);
+    const uint32_t go = elect_one();
+    constexpr uint32_t idesc_qk = umma_idesc_16(FP16, 256, 128, 0, 0);
+    constexpr uint32_t idesc_pv = umma_idesc_16(FP16, 256, 128, 0, 1);
+    const uint64_t qd = umma_desc_sw128(smem_u32(smem + L::kQ), 16), kd = umma_desc_sw128(smem_u32(smem + L::kK), 16),
+                   vd = umma_desc_sw128(smem_u32(smem + L::kV), 16);
+    volatile int2 *queue = reinterpret_cast<volatile int2 *>(smem + L::kQueue);
+    // Two cursors over the items' tiles: the scores run ahead of the output by up to three.  Items pass from one to the other
+    // through a queue, and records are given back at once.
+    int s_it = 0, s_left = 0, o_n = 0, o_t = 0, o_nk = 0;
+    uint32_t scored = 0, added = 0, items_in = 0, items_out = 0;         // tiles; items with keys
+    bool ok = true, more = true;                 // more: there may be tiles to score
+    while (ok) {
+        while (more && scored - added < static_cast<uint32_t>(kBuffers)) {
+            if (s_left == 0) {
+                const int slot = s_it % kRecords;
+                const uint32_t rec_bar = bars + (L::kBarRecFull + slot) * 8, rec_phase = (s_it / kRecords) & 1;
+                // While output is outstanding the next record may depend on it: it is looked for, not waited for.
+                if (scored != added) {
+                    if (!__all_sync(0xffffffffu, mbar_test_wait(rec_bar, rec_phase))) break;
+                } else if (!(ok = mbar_wait(rec_bar, rec_phase, abort_flag))) {
+                    break;
+                }
+                const volatile int *rec = reinterpret_cast<const int *>(smem + L::kRecs) + slot * kRecInts;
+                more = rec[kRecValid] != 0;
+                const int nk = rec[kRecNk];
+                s_left = more ? rec[kRecN] : 0;
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(bars + (L::kBarRecEmpty + slot) * 8);
+                    if (s_left > 0) {
+                        queue[items_in % 8].x = s_left;
+                        queue[items_in % 8].y = nk;
+                    }
+                }
+                __syncwarp();
+                ++s_it;
+                if (s_left == 0) continue;
+                if (!(ok = mbar_wait(bars + (L::kBarQFull + (items_in & 1)) * 8, (items_in >> 1) & 1, abort_flag))) break;
+                ++items_in;
+            }
+            // S(scored), into the buffer of the tile three before, whose product into O has been issued
+            const uint32_t at = scored % L::kSlots, buf = scored % kBuffers, qb = (items_in - 1) & 1;
+            if (!(ok = mbar_wait(bars + (L::kBarKFull + at) * 8, (scored / L::kSlots) & 1, abort_flag))) break;
+            tc_fence_after_sync();
+            const uint64_t qa = qd + static_cast<uint64_t>((qb * L::kQBytes) >> 4), kb = kd + static_cast<uint64_t>((at * L::kKBytes) >> 4);
+            if (go) {
+#pragma unroll
+                for (int s = 0; s < L::kDSlabs; ++s)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        umma_ss_pair_pred(tmem + buf * 128, qa + ((s * kSlab) >> 4) + 2 * k, kb + ((s * kHalfSlab) >> 4) + 2 * k, idesc_qk,
+                                          (s | k) ? 1u : 0u, 1u);
+            }
+            umma_commit_pair_pred(bars + (L::kBarS + buf) * 8, go);
+            umma_commit_pair_pred(bars + (L::kBarKEmpty + at) * 8, go);
+            if (--s_left == 0) umma_commit_pair_pred(bars + (L::kBarQEmpty + qb) * 8, go);
+            ++scored;
+        }
+        if (!ok || scored == added) break;       // (nothing outstanding: the records are at their end)
+        // O += P V of the next tile
+        if (o_t == o_n) {
+            o_n = queue[items_out % 8].x;
+            o_nk = queue[items_out % 8].y;
+            ++items_out;
+            o_t = 0;
+        }
+        const uint32_t at = added % L::kSlots, buf = added % kBuffers;
+        if (!(ok = mbar_wait(bars + (L::kBarVFull + at) * 8, (added / L::kSlots) & 1, abort_flag))) break;
+        // the weights of both CTAs are in tensor memory; O has been moved to a new reference where one was needed, and the last
+        // item's output has been read
+        if (!(ok = mbar_wait(bars + (L::kBarP + buf) * 8, (added / kBuffers) & 1, abort_flag))) break;
+        tc_fence_after_sync();
+        const int left = o_nk - o_t * 128, steps = left >= 128 ? 8 : (left + 15) >> 4;
+        const uint64_t v = vd + static_cast<uint64_t>((at * kSlab) >> 4);
+        const uint32_t p = tmem + buf * 128, acc = o_t > 0 ? 1u : 0u;
+        if (steps == 8) {
+            if (go) {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) umma_ts_pair_pred(tmem + kTmemO, p + k * 8, v + k * 128, idesc_pv, k ? 1u : acc, 1u);
+            }
+        } else {
+            for (int k = 0; k < steps; ++k) umma_ts_pair_pred(tmem + kTmemO, p + k * 8, v + k * 128, idesc_pv, k ? 1u : acc, go);
+        }
+        umma_commit_pair_pred(bars + (L::kBarPv + (added & 1)) * 8, go);
+        umma_commit_pair_pred(bars + (L::kBarVEmpty + at) * 8, go);
+        ++added;
+        if (++o_t == o_n) umma_commit_pair_pred(bars + L::kBarO * 8, go);
     }
     if (!ok && lane == 0) give_up(abort_flag, a.status, kStatusMmaWait);
 }
@@ -346,34 +403,39 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
     return r;
 }
 
+// Warpgroup `side` takes the tiles g with g % 2 == side of a CTA's sequence; its thread is a row (lane of tensor memory).  The
+// row's reference passes from tile to tile through shared memory; each warpgroup keeps its own part of the sum.
 template <int DQK, bool FP16>
-__device__ __forceinline__ void softmax_role(const PrefillArgs &a, uint8_t *smem, uint32_t tmem, volatile int *abort_flag, int warp, int lane) {
+__device__ __forceinline__ void softmax_role(const PrefillArgs &a, uint8_t *smem, uint32_t tmem, volatile int *abort_flag, int rank, int warp, int lane) {
     using L = Smem<DQK>;
     const uint32_t bars = smem_u32(smem + L::kBars);
-    const int half = warp >> 2, lane0 = (warp & 3) * 32;
-    const uint32_t s_addr = tmem + half * 128 + (static_cast<uint32_t>(lane0) << 16);
-    const uint32_t o_addr = s_addr - half * 128 + 256 + half * 128;
-    const int row = half * 128 + lane0 + lane;   // of the item
+    const int side = warp >> 2, quarter = warp & 3, lane_row = quarter * 32 + lane, row = rank * 128 + lane_row;
+    const uint32_t t_lane = tmem + (static_cast<uint32_t>(quarter * 32) << 16), o_addr = t_lane + kTmemO;
+    float *ref_at = reinterpret_cast<float *>(smem + L::kRef) + lane_row;
+    const uint32_t p_bar = map_rank(bars + L::kBarP * 8, 0);  // the even CTA's
+    float2 *sums = reinterpret_cast<float2 *>(smem + L::kSums) + lane_row;
     const float c = a.scale_log2;
-    uint32_t ns = 0, no = 0;
+    uint32_t tile = 0, n_out = 0;
+    bool failed = false;
+    // The two warps of a quarter meet at barriers: for each item, where they leave together if one of them has given up, and
+    // at its end, through which they go whatever happens.
     for (int it = 0;; ++it) {
         const int slot = it % kRecords;
-        if (!mbar_wait(bars + (L::kBarRecFull + slot) * 8, (it / kRecords) & 1, abort_flag)) break;
+        failed |= !mbar_wait(bars + (L::kBarRecFull + slot) * 8, (it / kRecords) & 1, abort_flag);
         const volatile int *rec = reinterpret_cast<const int *>(smem + L::kRecs) + slot * kRecInts;
-        const int valid = rec[kRecValid], n = rec[half ? kRecN1 : kRecN0], nk = rec[kRecNk], off = rec[kRecOff], rows = rec[kRecRows],
-                  head = rec[kRecHead], qrow = rec[kRecQRow];
+        const int valid = rec[kRecValid], n = rec[kRecN], nk = rec[kRecNk], off = rec[kRecOff], rows = rec[kRecRows], head = rec[kRecHead],
+                  qrow = rec[kRecQRow];
         __syncwarp();
         if (lane == 0) mbar_arrive(bars + (L::kBarRecEmpty + slot) * 8);
-        if (!valid) return;
-        const int lim = a.causal ? min(nk, off + row + 1) : nk;                    // keys that this row sees
-        const int lim_warp = a.causal ? min(nk, off + half * 128 + lane0 + 1) : nk; // ... and the warp's first row
+        if (named_bar_or(1 + quarter, 64, failed) || !valid) break;
+        const int lim = a.causal ? min(nk, off + row + 1) : nk;                        // keys that this row sees
+        const int lim_warp = a.causal ? min(nk, off + row - lane + 1) : nk;            // ... and the warp's first row
         float m = -INFINITY;                     // the reference, in log2 units
         uint64_t l2 = 0;                         // two partial sums
-        for (int t = 0; t < n; ++t, ++ns) {
-            if (!mbar_wait(bars + (L::kBarS + half) * 8, ns & 1, abort_flag)) {
-                if (lane == 0) give_up(abort_flag, a.status, kStatusSoftmaxWait);
-                return;
-            }
+        for (int t = 0; t < n; ++t, ++tile) {
+            if ((tile & 1) != static_cast<uint32_t>(side)) continue;
+            const uint32_t buf = tile % kBuffers, s_addr = t_lane + buf * 128;
+            failed |= !mbar_wait(bars + (L::kBarS + buf) * 8, (tile / kBuffers) & 1, abort_flag);
             tc_fence_after_sync();
             uint32_t s[128];
 #pragma unroll
@@ -391,22 +453,24 @@ __device__ __forceinline__ void softmax_role(const PrefillArgs &a, uint8_t *smem
             }
             float mx[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) mx[j] = __uint_as_float(s[j]);
+            for (int e = 0; e < 4; ++e) mx[e] = fmaxf(__uint_as_float(s[e]), __uint_as_float(s[4 + e]));
 #pragma unroll
-            for (int j = 4; j < 128; j += 8) {
+            for (int j = 8; j < 128; j += 8) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    mx[e] = fmaxf(mx[e], j + 4 + e < 128 ? fmaxf(__uint_as_float(s[j + e]), __uint_as_float(s[j + 4 + e])) : __uint_as_float(s[j + e]));
+                for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], fmaxf(__uint_as_float(s[j + e]), __uint_as_float(s[j + 4 + e])));
             }
             const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;
-            const bool move = top > m + 8.0f;
-            if (__any_sync(0xffffffffu, move)) {
-                const float to = move ? top : m;
-                const float f = move ? fast_exp2(m - to) : 1.0f;         // 0 for the row's first keys
-                m = to;
-                l2 = mul2(l2, pack2(f, f));
-                if (t > 0) {
-                    // every earlier product into O_i is complete: the scores of this block were issued behind them
+            // the reference as the tile before left it
+            if (tile > 0)
+                failed |= !mbar_wait(bars + (L::kBarRef + ((tile - 1) & 1) * 4 + quarter) * 8, ((tile - 1) >> 1) & 1, abort_flag);
+            const float now = t > 0 ? *ref_at : -INFINITY, to = top > now + 8.0f ? top : now;
+            if (t == 0 || __any_sync(0xffffffffu, to != m)) {
+                // (the warpgroup's first tile of an item, or one of the last two tiles moved a reference)
+                if (t > 0 && __any_sync(0xffffffffu, to != now)) {
+                    // everything before this tile has to be in O, nothing behind it can be
+                    failed |= !mbar_wait(bars + (L::kBarPv + ((tile - 1) & 1)) * 8, ((tile - 1) >> 1) & 1, abort_flag);
+                    tc_fence_after_sync();
+                    const float f = to == now ? 1.0f : fast_exp2(now - to);
 #pragma unroll 1
                     for (int j = 0; j < 128; j += 8) {
                         uint32_t o[8];
@@ -416,7 +480,13 @@ __device__ __forceinline__ void softmax_role(const PrefillArgs &a, uint8_t *smem
                         tmem_st_x8(o_addr + j, o);
                     }
                 }
+                *ref_at = to;
+                const float f = to == m ? 1.0f : fast_exp2(m - to);      // 0 for the warpgroup's first keys
+                l2 = mul2(l2, pack2(f, f));
+                m = to;
+                __syncwarp();
             }
+            if (lane == 0) mbar_arrive(bars + (L::kBarRef + (tile & 1) * 4 + quarter) * 8);
             const float ref = m == -INFINITY ? 0.0f : -m;
             const uint64_t c2 = pack2(c, c), ref2 = pack2(ref, ref);
             uint64_t la = l2, lb = 0;
@@ -439,31 +509,33 @@ __device__ __forceinline__ void softmax_role(const PrefillArgs &a, uint8_t *smem
             tmem_st_wait();
             tc_fence_before_sync();
             __syncwarp();
-            if (lane == 0) mbar_arrive(bars + (L::kBarP + half) * 8);
+            if (lane == 0) mbar_arrive_remote(p_bar + buf * 8);
         }
+        // the item's end: the warpgroups' sums under the later of their references (it only rises)
         float lx, ly;
         unpack2(l2, lx, ly);
-        const float l = lx + ly;
+        sums[side * 128] = make_float2(m, lx + ly);
+        named_bar_sync(1 + quarter, 64);
+        const float2 s0 = sums[0], s1 = sums[128];
+        named_bar_sync(1 + quarter, 64);
+        m = fmaxf(s0.x, s1.x);
+        const float l = m == -INFINITY ? s0.y + s1.y : s0.y * fast_exp2(s0.x - m) + s1.y * fast_exp2(s1.x - m);     // 0, or NaN from NaN
         const bool mine = row < rows;
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        if (mine && a.lse != nullptr) a.lse[head * a.lse_hs + qrow + row] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
-        uint16_t *dst = static_cast<uint16_t *>(a.out) + (qrow + row) * a.o_ts + head * a.o_hs;
+        if (mine && side == 0 && a.lse != nullptr) a.lse[head * a.lse_hs + qrow + row] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
+        uint16_t *dst = static_cast<uint16_t *>(a.out) + (qrow + row) * a.o_ts + head * a.o_hs + side * 64;
         if (n > 0) {
-            if (!mbar_wait(bars + (L::kBarO + half) * 8, no & 1, abort_flag)) {
-                if (lane == 0) give_up(abort_flag, a.status, kStatusEpilogueWait);
-                return;
-            }
-            ++no;
+            failed |= !mbar_wait(bars + L::kBarO * 8, n_out++ & 1, abort_flag);
             tc_fence_after_sync();
         }
 #pragma unroll
-        for (int j = 0; j < 128; j += 32) {
+        for (int j = 0; j < 64; j += 32) {
             uint32_t o[32];
             if (n > 0) {
-                tmem_ld_x32_nowait(o_addr + j, o);
+                tmem_ld_x32_nowait(o_addr + side * 64 + j, o);
                 tmem_ld_wait();
             }
-            if (mine) {
+            if (mine && !failed) {
 #pragma unroll
                 for (int e = 0; e < 32; e += 8) {
                     uint32_t w[4];
@@ -474,15 +546,19 @@ __device__ __forceinline__ void softmax_role(const PrefillArgs &a, uint8_t *smem
                 }
             }
         }
-        tc_fence_before_sync();                  // the next item's first product comes behind this warp's next arrival
+        // whichever of the two hands over the next item's first weights, both have read this one's output
+        tc_fence_before_sync();
+        named_bar_sync(1 + quarter, 64);
+        tc_fence_after_sync();
     }
+    if (failed && lane == 0) give_up(abort_flag, a.status, kStatusSoftmaxWait);
 }
 
 template <int DQK, bool FP16>
 __global__ void __launch_bounds__(kThreads, 1) dense_prefill_kernel(const __grid_constant__ PrefillArgs a) {
     extern __shared__ __align__(1024) uint8_t smem[];
     using L = Smem<DQK>;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, rank = static_cast<int>(cluster_rank());
     volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + L::kMisc);
     const uint32_t bars = smem_u32(smem + L::kBars);
     if ((smem_u32(smem) & 1023u) != 0u) {        // the swizzled slabs need it
@@ -490,43 +566,42 @@ __global__ void __launch_bounds__(kThreads, 1) dense_prefill_kernel(const __grid
         return;
     }
     if (tid == 0) {
-        for (int i = 0; i < L::kRing; ++i) {
-            mbar_init(bars + (L::kBarFull + i) * 8, 1);
-            mbar_init(bars + (L::kBarEmpty + i) * 8, 1);
-        }
-        mbar_init(bars + L::kBarQFull * 8, 1);
-        mbar_init(bars + L::kBarQEmpty * 8, 1);
-        for (int i = 0; i < 2; ++i) {
-            mbar_init(bars + (L::kBarS + i) * 8, 1);
-            mbar_init(bars + (L::kBarP + i) * 8, 4);
-            mbar_init(bars + (L::kBarO + i) * 8, 1);
-        }
-        for (int i = 0; i < kRecords; ++i) {
-            mbar_init(bars + (L::kBarRecFull + i) * 8, 1);
-            mbar_init(bars + (L::kBarRecEmpty + i) * 8, 9);
-        }
+        const auto init = [&](int first, int n, int count) {
+            for (int i = 0; i < n; ++i) mbar_init(bars + (first + i) * 8, count);
+        };
+        init(L::kBarQFull, 4, 1);                // and kBarQEmpty
+        init(L::kBarKFull, 2 * L::kSlots, 1);    // and kBarKEmpty
+        init(L::kBarVFull, L::kSlots, 2);        // both CTAs' loaders
+        init(L::kBarVEmpty, L::kSlots, 1);
+        init(L::kBarS, kBuffers, 1);
+        init(L::kBarP, kBuffers, 8);             // four warps of each CTA
+        init(L::kBarPv, 2, 1);
+        init(L::kBarO, 1, 1);
+        init(L::kBarRef, 8, 1);
+        init(L::kBarTail, 1, 1);
+        init(L::kBarRecFull, kRecords, 1);
+        init(L::kBarRecEmpty, kRecords, rank == 0 ? 10 : 9);
         *abort_flag = 0;
         mbar_init_fence();
     }
-    if (warp == 8) tmem_alloc(smem_u32(smem + L::kMisc + 8), 512);
+    if (warp == 8) tmem_alloc_pair(smem_u32(smem + L::kMisc + 8), 512);
     tc_fence_before_sync();
-    __syncthreads();
+    cluster_sync_all();                          // also: the other CTA's barriers are there
     tc_fence_after_sync();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(smem + L::kMisc + 8);
     if (warp < 8) {
         regs_inc<kRegsSoftmax>();
-        softmax_role<DQK, FP16>(a, smem, tmem, abort_flag, warp, lane);
+        softmax_role<DQK, FP16>(a, smem, tmem, abort_flag, rank, warp, lane);
     } else {
         regs_dec<kRegsOther>();
-        if (warp == 8) mma_role<DQK, FP16>(a, smem, tmem, abort_flag, lane);
-        else if (warp == 9) loader_role<DQK>(a, smem, abort_flag, lane);
+        if (warp == 8 && rank == 0) mma_role<DQK, FP16>(a, smem, tmem, abort_flag, lane);
+        else if (warp == 9) qk_loader_role<DQK>(a, smem, abort_flag, rank, lane);
+        else if (warp == 10) v_loader_role<DQK>(a, smem, abort_flag, rank, lane);
     }
     tc_fence_before_sync();
-    __syncthreads();
-    if (warp == 8) {
-        tmem_relinquish();
-        tmem_dealloc(tmem, 512);
-    }
+    __syncwarp();
+    cluster_sync_all();                          // nothing of this CTA's is used by the other any more
+    if (warp == 8) tmem_free_pair(tmem, 512);
 }
 
 template <int DQK, bool FP16>
@@ -534,8 +609,18 @@ int launch(PrefillArgs &a, unsigned grid, cudaStream_t stream) {
     static KernelSetup setup;
     const int rc = setup.get(reinterpret_cast<const void *>(&dense_prefill_kernel<DQK, FP16>), Smem<DQK>::kBytes, &a.status, kRegsLaunch);
     if (rc != 0) return rc;
-    dense_prefill_kernel<DQK, FP16><<<grid, kThreads, Smem<DQK>::kBytes, stream>>>(a);
-    return static_cast<int>(cudaGetLastError());
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = Smem<DQK>::kBytes;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = 2;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return static_cast<int>(cudaLaunchKernelEx(&cfg, dense_prefill_kernel<DQK, FP16>, a));
 }
 
 }  // namespace
@@ -547,7 +632,7 @@ int launch_dense_prefill(const smla_prefill_params_t &p, int sm_count, cudaStrea
         return SMLA_EINVAL;
     // without keys no item has a key block, and the maps of k and v are never used
     if (p.total_k > 0 &&
-        (!make_slab_map(&a.k_map, fp16, p.k, p.head_dim, p.total_k, p.num_kv_heads, p.k_token_stride * 2, p.k_head_stride * 2, 128) ||
+        (!make_slab_map(&a.k_map, fp16, p.k, p.head_dim, p.total_k, p.num_kv_heads, p.k_token_stride * 2, p.k_head_stride * 2, 64) ||
          !make_slab_map(&a.v_map, fp16, p.v, 128, p.total_k, p.num_kv_heads, p.v_token_stride * 2, p.v_head_stride * 2, 128)))
         return SMLA_EINVAL;
     a.out = p.out;
@@ -569,7 +654,7 @@ int launch_dense_prefill(const smla_prefill_params_t &p, int sm_count, cudaStrea
     a.scale_log2 = std::max(c < 0.0f ? -c : c, 1e-35f);
     // each sequence adds at most one item that is not full
     const int64_t items = (p.total_q / 256 + p.batch) * p.num_heads;
-    const unsigned grid = static_cast<unsigned>(std::min<int64_t>(items, sm_count));
+    const unsigned grid = 2 * static_cast<unsigned>(std::min<int64_t>(items, sm_count / 2));
     if (p.head_dim == 192) return fp16 ? launch<192, true>(a, grid, stream) : launch<192, false>(a, grid, stream);
     return fp16 ? launch<128, true>(a, grid, stream) : launch<128, false>(a, grid, stream);
 }
