@@ -15,11 +15,14 @@
 //   S(g) = Q K(g)^T  -> one of three buffers of 128 columns in tensor memory
 //   P(g) = exp(S(g) - m)  -> 16-bit, written over S(g) (64 columns)
 //   O += P(g) V(g)  -> 128 columns
-// The products are issued in the order S(g + 2), O(g): the weights of a tile have the time of two tiles' products to be
-// computed in, and two warpgroups take turns at the tiles, so that a weight computation (about 2100 cycles for a tile, one
-// row per thread) may take nearly twice as long as the products of a tile (1280 cycles at 192 dims).  With one CTA per
-// item, S in one buffer for each half of the rows, the chain scores - weights - output - next scores bounded it: 1.05
-// PFLOP/s on a prompt of 16384 tokens.
+// Three tiles are scored ahead of the output, so the weights of a tile have the time of two tiles' products to be computed
+// in, and two warpgroups take turns at the tiles: a weight computation (about 2100 cycles for a tile, one row per thread)
+// may take nearly twice as long as the products of a tile (1280 cycles at 192 dims).
+// What bounds it: tensor work, at 88 % while a long item runs (1460 cycles a tile: the chain weights - output - score of the
+// tile three on takes a little longer than three tiles' products).  8192 causal tokens of 37 heads: 594 us with 192 dims
+// (1.34 PFLOP/s), 529 us with 128 (1.20).  Measured against it: one CTA per item, S in one buffer for each half of the rows,
+// 675 and 580 us; weights in buffers of their own beside S (a fourth wait and narrower stores) 660 and 587; weights handed
+// over in two pieces 602 and 530; the rows' reference through mbarriers in place of named ones 600 and 542.
 // K and V arrive by TMA as slabs of 64 dims with the 128-byte swizzle: of K the rows of 64 keys (its half of N), of V all
 // 128 keys of 64 of the dims (its half of N there).  A slab read K-major gives K for the first product, MN-major V for the
 // second.  Sharing B halves the fills: with both operands from shared memory one CTA's products alone (M = N = 128) take all
@@ -78,7 +81,7 @@ struct Smem {
     static constexpr int kBars = kV + kSlots * kSlab;
     static constexpr int kBarQFull = 0, kBarQEmpty = 2, kBarKFull = 4, kBarKEmpty = kBarKFull + kSlots, kBarVFull = kBarKEmpty + kSlots,
                          kBarVEmpty = kBarVFull + kSlots, kBarS = kBarVEmpty + kSlots, kBarP = kBarS + kBuffers, kBarPv = kBarP + kBuffers,
-                         kBarO = kBarPv + 2, kBarRef = kBarO + 1, kBarTail = kBarRef + 8, kBarRecFull = kBarTail + 1,
+                         kBarO = kBarPv + 2, kBarTail = kBarO + 1, kBarRecFull = kBarTail + 1,
                          kBarRecEmpty = kBarRecFull + kRecords, kNumBars = kBarRecEmpty + kRecords;
     static constexpr int kRecs = kBars + kNumBars * 8;
     static constexpr int kRef = kRecs + kRecords * kRecInts * 4;         // the rows' reference
@@ -299,6 +302,11 @@ __device__ __forceinline__ void v_loader_role(const PrefillArgs &a, uint8_t *sme
 }
 
 // ------------------------------------------------------------------ products (the even CTA, for both)
+// Two barriers, looked at together first: a look takes this warp over 100 cycles, but they overlap.
+__device__ __forceinline__ bool wait_both(uint32_t b0, uint32_t p0, uint32_t b1, uint32_t p1, volatile int *abort_flag) {
+    const bool x = mbar_test_wait(b0, p0), y = mbar_test_wait(b1, p1);
+    return (x && y) || (mbar_wait(b0, p0, abort_flag) && mbar_wait(b1, p1, abort_flag));
+}
 template <int DQK, bool FP16>
 __device__ __forceinline__ void mma_role(const PrefillArgs &a, uint8_t *smem, uint32_t tmem, volatile int *abort_flag, int lane) {
     using L = Smem<DQK>;
@@ -314,82 +322,100 @@ __device__ __forceinline__ void mma_role(const PrefillArgs &a, uint8_t *smem, ui
     int s_it = 0, s_left = 0, o_n = 0, o_t = 0, o_nk = 0;
     uint32_t scored = 0, added = 0, items_in = 0, items_out = 0;         // tiles; items with keys
     bool ok = true, more = true;                 // more: there may be tiles to score
-    while (ok) {
-        while (more && scored - added < static_cast<uint32_t>(kBuffers)) {
-            if (s_left == 0) {
-                const int slot = s_it % kRecords;
-                const uint32_t rec_bar = bars + (L::kBarRecFull + slot) * 8, rec_phase = (s_it / kRecords) & 1;
-                // While output is outstanding the next record may depend on it: it is looked for, not waited for.
-                if (scored != added) {
-                    if (!__all_sync(0xffffffffu, mbar_test_wait(rec_bar, rec_phase))) break;
-                } else if (!(ok = mbar_wait(rec_bar, rec_phase, abort_flag))) {
-                    break;
+
+    // Finds the next tile to score and waits for its operands.  While output is outstanding the next record may depend on it:
+    // it is then looked for, not waited for.
+    const auto find_tile = [&] {
+        while (more && s_left == 0) {
+            const int slot = s_it % kRecords;
+            const uint32_t rec_bar = bars + (L::kBarRecFull + slot) * 8, rec_phase = (s_it / kRecords) & 1;
+            if (scored != added) {
+                if (!__all_sync(0xffffffffu, mbar_test_wait(rec_bar, rec_phase))) return false;
+            } else if (!(ok = mbar_wait(rec_bar, rec_phase, abort_flag))) {
+                return false;
+            }
+            const volatile int *rec = reinterpret_cast<const int *>(smem + L::kRecs) + slot * kRecInts;
+            more = rec[kRecValid] != 0;
+            const int nk = rec[kRecNk];
+            s_left = more ? rec[kRecN] : 0;
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(bars + (L::kBarRecEmpty + slot) * 8);
+                if (s_left > 0) {
+                    queue[items_in % 8].x = s_left;
+                    queue[items_in % 8].y = nk;
                 }
-                const volatile int *rec = reinterpret_cast<const int *>(smem + L::kRecs) + slot * kRecInts;
-                more = rec[kRecValid] != 0;
-                const int nk = rec[kRecNk];
-                s_left = more ? rec[kRecN] : 0;
-                __syncwarp();
-                if (lane == 0) {
-                    mbar_arrive(bars + (L::kBarRecEmpty + slot) * 8);
-                    if (s_left > 0) {
-                        queue[items_in % 8].x = s_left;
-                        queue[items_in % 8].y = nk;
-                    }
-                }
-                __syncwarp();
-                ++s_it;
-                if (s_left == 0) continue;
-                if (!(ok = mbar_wait(bars + (L::kBarQFull + (items_in & 1)) * 8, (items_in >> 1) & 1, abort_flag))) break;
+            }
+            __syncwarp();
+            ++s_it;
+            if (s_left > 0) {
+                if (!(ok = mbar_wait(bars + (L::kBarQFull + (items_in & 1)) * 8, (items_in >> 1) & 1, abort_flag))) return false;
                 ++items_in;
             }
-            // S(scored), into the buffer of the tile three before, whose product into O has been issued
-            const uint32_t at = scored % L::kSlots, buf = scored % kBuffers, qb = (items_in - 1) & 1;
-            if (!(ok = mbar_wait(bars + (L::kBarKFull + at) * 8, (scored / L::kSlots) & 1, abort_flag))) break;
-            tc_fence_after_sync();
-            const uint64_t qa = qd + static_cast<uint64_t>((qb * L::kQBytes) >> 4), kb = kd + static_cast<uint64_t>((at * L::kKBytes) >> 4);
-            if (go) {
-#pragma unroll
-                for (int s = 0; s < L::kDSlabs; ++s)
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        umma_ss_pair_pred(tmem + buf * 128, qa + ((s * kSlab) >> 4) + 2 * k, kb + ((s * kHalfSlab) >> 4) + 2 * k, idesc_qk,
-                                          (s | k) ? 1u : 0u, 1u);
-            }
-            umma_commit_pair_pred(bars + (L::kBarS + buf) * 8, go);
-            umma_commit_pair_pred(bars + (L::kBarKEmpty + at) * 8, go);
-            if (--s_left == 0) umma_commit_pair_pred(bars + (L::kBarQEmpty + qb) * 8, go);
-            ++scored;
         }
-        if (!ok || scored == added) break;       // (nothing outstanding: the records are at their end)
-        // O += P V of the next tile
+        if (!more || !(ok = mbar_wait(bars + (L::kBarKFull + scored % L::kSlots) * 8, (scored / L::kSlots) & 1, abort_flag))) return false;
+        tc_fence_after_sync();
+        return true;
+    };
+    // S(scored) = Q K^T, into the buffer of the tile three before, whose product into O has been issued
+    const auto score = [&] {
+        const uint32_t at = scored % L::kSlots, buf = scored % kBuffers, qb = (items_in - 1) & 1;
+        const uint64_t qa = qd + static_cast<uint64_t>((qb * L::kQBytes) >> 4), kb = kd + static_cast<uint64_t>((at * L::kKBytes) >> 4);
+        if (go) {
+#pragma unroll
+            for (int s = 0; s < L::kDSlabs; ++s)
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    umma_ss_pair_pred(tmem + buf * 128, qa + ((s * kSlab) >> 4) + 2 * k, kb + ((s * kHalfSlab) >> 4) + 2 * k, idesc_qk,
+                                      (s | k) ? 1u : 0u, 1u);
+        }
+        umma_commit_pair_pred(bars + (L::kBarS + buf) * 8, go);
+        umma_commit_pair_pred(bars + (L::kBarKEmpty + at) * 8, go);
+        if (--s_left == 0) umma_commit_pair_pred(bars + (L::kBarQEmpty + qb) * 8, go);
+        ++scored;
+    };
+    // Three tiles are scored ahead, the next one right behind the product into O that frees its buffer.
+    while (scored < static_cast<uint32_t>(kBuffers) && find_tile()) score();
+    uint32_t at = 0, buf = 0, v_phase = 0, p_phase = 0;      // of tile `added`
+    while (ok && scored != added) {
         if (o_t == o_n) {
             o_n = queue[items_out % 8].x;
             o_nk = queue[items_out % 8].y;
             ++items_out;
             o_t = 0;
         }
-        const uint32_t at = added % L::kSlots, buf = added % kBuffers;
-        if (!(ok = mbar_wait(bars + (L::kBarVFull + at) * 8, (added / L::kSlots) & 1, abort_flag))) break;
-        // the weights of both CTAs are in tensor memory; O has been moved to a new reference where one was needed, and the last
-        // item's output has been read
-        if (!(ok = mbar_wait(bars + (L::kBarP + buf) * 8, (added / kBuffers) & 1, abort_flag))) break;
-        tc_fence_after_sync();
-        const int left = o_nk - o_t * 128, steps = left >= 128 ? 8 : (left + 15) >> 4;
+        // O += P V of the next tile
+        const int left = o_nk - o_t * 128;
         const uint64_t v = vd + static_cast<uint64_t>((at * kSlab) >> 4);
         const uint32_t p = tmem + buf * 128, acc = o_t > 0 ? 1u : 0u;
-        if (steps == 8) {
+        // V, and the weights of both CTAs in tensor memory; O has been moved to a new reference where one was needed, and the last
+        // item's output has been read
+        if (!(ok = wait_both(bars + (L::kBarVFull + at) * 8, v_phase, bars + (L::kBarP + buf) * 8, p_phase, abort_flag))) break;
+        tc_fence_after_sync();
+        if (left > 112) {
             if (go) {
 #pragma unroll
                 for (int k = 0; k < 8; ++k) umma_ts_pair_pred(tmem + kTmemO, p + k * 8, v + k * 128, idesc_pv, k ? 1u : acc, 1u);
             }
         } else {
-            for (int k = 0; k < steps; ++k) umma_ts_pair_pred(tmem + kTmemO, p + k * 8, v + k * 128, idesc_pv, k ? 1u : acc, go);
+            for (int k = 0; k * 16 < left; ++k) umma_ts_pair_pred(tmem + kTmemO, p + k * 8, v + k * 128, idesc_pv, k ? 1u : acc, go);
         }
-        umma_commit_pair_pred(bars + (L::kBarPv + (added & 1)) * 8, go);
-        umma_commit_pair_pred(bars + (L::kBarVEmpty + at) * 8, go);
         ++added;
         if (++o_t == o_n) umma_commit_pair_pred(bars + L::kBarO * 8, go);
+        if (find_tile()) score();
+        if (!ok) break;
+        umma_commit_pair_pred(bars + (L::kBarPv + ((added - 1) & 1)) * 8, go);
+        umma_commit_pair_pred(bars + (L::kBarVEmpty + at) * 8, go);
+        if (++at == L::kSlots) {
+            at = 0;
+            v_phase ^= 1;
+        }
+        if (++buf == kBuffers) {
+            buf = 0;
+            p_phase ^= 1;
+        }
+        // the last tiles of an item whose successor was not there yet
+        while (scored - added < static_cast<uint32_t>(kBuffers) && find_tile()) score();
     }
     if (!ok && lane == 0) give_up(abort_flag, a.status, kStatusMmaWait);
 }
@@ -418,7 +444,7 @@ __device__ __forceinline__ void softmax_role(const PrefillArgs &a, uint8_t *smem
     uint32_t tile = 0, n_out = 0;
     bool failed = false;
     // The two warps of a quarter meet at barriers: for each item, where they leave together if one of them has given up, and
-    // at its end, through which they go whatever happens.
+    // at its tiles and its end, through which they go whatever happens.
     for (int it = 0;; ++it) {
         const int slot = it % kRecords;
         failed |= !mbar_wait(bars + (L::kBarRecFull + slot) * 8, (it / kRecords) & 1, abort_flag);
@@ -461,8 +487,7 @@ __device__ __forceinline__ void softmax_role(const PrefillArgs &a, uint8_t *smem
             }
             const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;
             // the reference as the tile before left it
-            if (tile > 0)
-                failed |= !mbar_wait(bars + (L::kBarRef + ((tile - 1) & 1) * 4 + quarter) * 8, ((tile - 1) >> 1) & 1, abort_flag);
+            if (tile > 0) named_bar_sync(6 + quarter * 2 - side, 64);
             const float now = t > 0 ? *ref_at : -INFINITY, to = top > now + 8.0f ? top : now;
             if (t == 0 || __any_sync(0xffffffffu, to != m)) {
                 // (the warpgroup's first tile of an item, or one of the last two tiles moved a reference)
@@ -486,7 +511,7 @@ __device__ __forceinline__ void softmax_role(const PrefillArgs &a, uint8_t *smem
                 m = to;
                 __syncwarp();
             }
-            if (lane == 0) mbar_arrive(bars + (L::kBarRef + (tile & 1) * 4 + quarter) * 8);
+            named_bar_arrive(5 + quarter * 2 + side, 64);    // the warp with the next tile's rows waits there
             const float ref = m == -INFINITY ? 0.0f : -m;
             const uint64_t c2 = pack2(c, c), ref2 = pack2(ref, ref);
             uint64_t la = l2, lb = 0;
@@ -551,6 +576,7 @@ __device__ __forceinline__ void softmax_role(const PrefillArgs &a, uint8_t *smem
         named_bar_sync(1 + quarter, 64);
         tc_fence_after_sync();
     }
+    if (tile > 0 && (tile & 1) == static_cast<uint32_t>(side)) named_bar_sync(6 + quarter * 2 - side, 64);      // the last arrival's
     if (failed && lane == 0) give_up(abort_flag, a.status, kStatusSoftmaxWait);
 }
 
@@ -577,7 +603,6 @@ __global__ void __launch_bounds__(kThreads, 1) dense_prefill_kernel(const __grid
         init(L::kBarP, kBuffers, 8);             // four warps of each CTA
         init(L::kBarPv, 2, 1);
         init(L::kBarO, 1, 1);
-        init(L::kBarRef, 8, 1);
         init(L::kBarTail, 1, 1);
         init(L::kBarRecFull, kRecords, 1);
         init(L::kBarRecEmpty, kRecords, rank == 0 ? 10 : 9);

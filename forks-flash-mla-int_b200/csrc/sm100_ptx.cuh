@@ -117,6 +117,10 @@ __device__ __forceinline__ void tc_fence_after_sync() {
 __device__ __forceinline__ void named_bar_sync(int id, int nthreads) {
     asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(nthreads) : "memory");
 }
+// The producer's side of a named barrier: counted, not waited.
+__device__ __forceinline__ void named_bar_arrive(int id, int nthreads) {
+    asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(nthreads) : "memory");
+}
 // Barrier + OR-reduction of a predicate over the participating threads.
 __device__ __forceinline__ bool named_bar_or(int id, int nthreads, bool pred) {
     uint32_t r;
@@ -243,17 +247,6 @@ __device__ __forceinline__ void tmem_ld_x32_nowait(uint32_t taddr, uint32_t *r) 
         : "memory");
 }
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t *r) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
-        :
-        : "r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
-          "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]),
-          "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]),
-          "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-        : "memory");
-}
 
 // ----------------------------------------------------------------------------- packed fp32 pairs
 __device__ __forceinline__ uint64_t pack2(float lo, float hi) {
@@ -336,20 +329,6 @@ __device__ __forceinline__ void umma_bf16_ss_pred(uint32_t d_tmem, uint64_t a_de
         "}"
         :
         : "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(go)
-        : "memory");
-}
-// The same with the A operand in tensor memory (lane = row, two 16-bit elements of K to a column).
-__device__ __forceinline__ void umma_f16_ts_pred(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
-                                                 uint32_t accumulate, uint32_t go) {
-    asm volatile(
-        "{\n\t"
-        ".reg .pred p, g;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "setp.ne.b32 g, %5, 0;\n\t"
-        "@g tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
-        "}"
-        :
-        : "r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(go)
         : "memory");
 }
 // Arrive on an mbarrier once every tcgen05 operation this thread issued so far has completed; issued by
