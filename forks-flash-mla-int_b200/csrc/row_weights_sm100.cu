@@ -7,17 +7,23 @@
 // lse is known, every term is at most 1.  Under the causal mask position i sees the rows r < len - (s_q - 1 - i), so a
 // row is seen by the columns c >= max(0, r - len + s_q) H: one threshold per lane.
 //
-// Two forms, by the number of columns C = s_q H (both persistent, one CTA per SM, tiles of 128 rows in contiguous ranges):
-//   C <= 128 (a decode step)  bound by reading the rows once.  K and Q slabs [rows][64 dims] stream through one ring of
-//            stages; Q (N x 64 dims a stage) is fetched again for each tile, from L2: N / 128 of the rows' bytes.
-//   C > 128 (a window)        bound by the tensor pipe.  The tile's rows stay in shared memory (147 KB) while the columns
-//            pass in blocks of 256 through the ring; the next tile's slabs replace the rows as the last block leaves them.
+// Two forms, by the number of columns C = s_q H (both persistent):
+//   C <= 128 (a decode step)  one CTA per SM, tiles of 128 rows in contiguous ranges.  Bound by reading the rows once.  K and Q
+//            slabs [rows][64 dims] stream through one ring of stages; Q (N x 64 dims a stage) is fetched again for each tile,
+//            from L2: N / 128 of the rows' bytes.  128 sequences of 4096 rows, 16 columns: 107 us, 5.7 TB/s of rows.
+//   C > 128 (a window)        pairs of CTAs that multiply as one (M = 256, half of the columns in each CTA's shared memory).
+//            The rows of a pair's tile stay in shared memory (147 KB each) while the columns pass in blocks of 256 through the
+//            ring; the next tile's slabs replace the rows as the last block leaves them.  With scratch the blocks of all tiles
+//            are dealt out evenly, and tiles that are cut are joined by a second kernel.  8192 columns, 28939 rows: 213 us, 1.28
+//            PFLOP/s (single CTAs with blocks of 128: 254 us).  Bound by the feed of columns: each pair takes 295 KB a block
+//            from L2, 6 TB/s over all, and 64 KB in flight are what the rows leave room for.
 // Roles (384 threads): warps 0-3 and 4-7 take turns at the score blocks (two accumulators), warp 8 issues the MMAs, warp
 // 9 finds the tiles and loads.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <algorithm>
+#include <cmath>
 #include <cstdint>
 
 #include "sm100_ptx.cuh"
@@ -42,6 +48,7 @@ struct WeightsArgs {
     int width, accumulate, batch, s_q, heads, columns, causal, k_slabs;
     int num_blocks, page, box_rows, max_blocks;
     float scale_log2;
+    float start, turn;                           // B and 8/3 B, see Smem
     // RES with scratch: the blocks of columns of all tiles are dealt out, and a tile that is cut leaves its sums here, 2 slots
     // of 128 per CTA (the end of a tile begun by a CTA before, the begin of one ended by a CTA behind), each with {sequence,
     // first row, first block, end block}
@@ -51,20 +58,30 @@ struct WeightsArgs {
 };
 
 // RES: the rows stay while the columns pass.  N: columns of a score block.
-// A score is a sum over nine (eight) slabs of 64 dims.  The tensor pipe cuts off what an addition leaves below the
-// accumulator's last bit, which over 36 additions to a sum of size 200 makes 5e-6 of a weight.  Where tensor memory has
-// room the slabs go to several accumulators that are added up with proper rounding: each is smaller and takes fewer
-// additions (one sequence, 16 columns: 4.5e-6 -> see kGroups).
+// A score is a sum over nine (eight) slabs of 64 dims in 36 steps.  The tensor pipe rounds a step's sum toward zero, always
+// to the side where it makes the score smaller: 4e-6 of a weight whose score is 6.
+// Up to 32 columns: tensor memory has room for an accumulator for each slab or two, which the sum warps add up with proper
+// rounding; their signs vary (one sequence, 16 columns: 4.5e-6 -> 3e-7).
+// More: a score starts at B (the scale's sign), and after half of its steps 8/3 B is taken off, so that it goes on from -5/3 B.
+// B = 1.125 2^j, with 2^j times the scale between 8 and 16: for scores up to 7, which have the weight, the sum then stays
+// between 2^j and 2^(j+1) in size, and the errors of the halves are the same on average, with opposite signs.  What is left
+// of a score, 2.7e-6, varies from column to column and averages out in the sums (64 query positions of 128 heads: 3.7e-6 ->
+// 2.3e-7).  Scores of other sizes fare as without B.  Both offsets are products of their own, of constant operands: 38 steps
+// for 36.
 template <bool RES, int N>
 struct Smem {
-    static constexpr int kPerGroup = RES ? 9 : N == 16 ? 1 : N == 32 ? 2 : N == 64 ? 3 : 5;      // slabs of an accumulator
+    static constexpr bool kBalanced = N >= 64;
+    static constexpr int kPerGroup = N == 16 ? 1 : N == 32 ? 2 : 9;      // slabs of an accumulator
     static constexpr int kGroups = (9 + kPerGroup - 1) / kPerGroup;
     static constexpr int kQSlab = (RES ? N / 2 : N) * 128;               // a CTA of a pair has half of the columns
     static constexpr int kStage = RES ? kQSlab : kSlab + kQSlab;
     static constexpr int kStages = RES ? 4 : (208 * 1024 / kStage < 12 ? 208 * 1024 / kStage : 12);
     static constexpr int kResident = RES ? 9 : 0;
     static constexpr int kRingAt = kResident * kSlab;
-    static constexpr int kLse = kRingAt + kStages * kStage;              // two buffers of N floats
+    static constexpr int kOnes = kRingAt + kStages * kStage;             // kBalanced: [128 rows][16 dims], 1 in two dims of each row
+    static constexpr int kStart = kOnes + (kBalanced ? 128 * 32 : 0);    // ... and as many columns as a slab of Q: start / 2 there
+    static constexpr int kTurn = kStart + (kBalanced ? kQSlab / 4 : 0);  // ... -turn / 2 there
+    static constexpr int kLse = kTurn + (kBalanced ? kQSlab / 4 : 0);    // two buffers of N floats
     static constexpr int kSums = kLse + 2 * N * 4;                       // RES: the second group's sums of a tile
     static constexpr int kBars = kSums + 128 * 4;
     static constexpr int kBarFull = 0, kBarEmpty = kStages, kBarKFull = 2 * kStages, kBarKEmpty = kBarKFull + kResident,
@@ -216,11 +233,18 @@ __device__ __forceinline__ void mma_role(const WeightsArgs &a, uint8_t *smem, ui
     const uint32_t bars = smem_u32(smem + L::kBars), ring = smem_u32(smem + L::kRingAt);
     const uint32_t go = elect_one();
     constexpr uint32_t idesc = umma_idesc_bf16(RES ? 256 : 128, N, 0, 0);
+    const auto multiply = [&](uint32_t d, uint64_t x, uint64_t y, uint32_t add) {
+        if constexpr (RES) umma_ss_pair_pred(d, x, y, idesc, add, 1u);
+        else umma_bf16_ss_pred(d, x, y, idesc, add, 1u);
+    };
     const auto commit = [&](uint32_t bar) {
         if constexpr (RES) umma_commit_pair_pred(bar, go);
         else umma_commit_pred(bar, go);
     };
     const uint64_t kd = umma_desc_sw128(RES ? smem_u32(smem) : ring, 16), qd = umma_desc_sw128(ring + (RES ? 0 : kSlab), 16);
+    // constant operands: all groups of 8 elements are alike
+    const uint64_t ones = umma_desc(smem_u32(smem + L::kOnes), 128, 256), start = umma_desc(smem_u32(smem + L::kStart), 128, 256),
+                   turn = umma_desc(smem_u32(smem + L::kTurn), 128, 256);
     uint32_t st = 0, n_blocks = 0;
     bool ok = true;
     for (int it = 0; ok; ++it) {
@@ -234,7 +258,10 @@ __device__ __forceinline__ void mma_role(const WeightsArgs &a, uint8_t *smem, ui
         for (int cb = cb0; cb < cb1 && ok; ++cb, ++n_blocks) {
             const int buf = n_blocks & 1;
             const uint32_t s_free = bars + (L::kBarSFree + buf) * 8, s_phase = ((n_blocks >> 1) & 1) ^ 1;
-            if (!(ok = RES ? mbar_wait_cluster(s_free, s_phase, abort_flag) : mbar_wait(s_free, s_phase, abort_flag))) break;
+            if (!(ok = mbar_wait(s_free, s_phase, abort_flag))) break;
+            tc_fence_after_sync();
+            const uint32_t d0 = tmem + buf * L::kGroups * N;
+            if (L::kBalanced && go) multiply(d0, ones, start, 0u);
             for (int s = 0; s < a.k_slabs; ++s, ++st) {
                 if (RES && cb == cb0 && !(ok = mbar_wait(bars + (L::kBarKFull + s) * 8, it & 1, abort_flag))) break;
                 const uint32_t at = st % L::kStages;
@@ -242,11 +269,14 @@ __device__ __forceinline__ void mma_role(const WeightsArgs &a, uint8_t *smem, ui
                 tc_fence_after_sync();
                 const uint64_t ka = kd + static_cast<uint64_t>((RES ? s * kSlab : at * L::kStage) >> 4);
                 const uint64_t qb = qd + static_cast<uint64_t>((at * L::kStage) >> 4);
+                if (go) {
+                    const uint32_t d = d0 + s / L::kPerGroup * N;
+                    const int half = 2 * a.k_slabs - 4 * s;      // products of this slab before the turn, where it is among them
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const uint32_t d = tmem + (buf * L::kGroups + s / L::kPerGroup) * N, add = s % L::kPerGroup || k ? 1u : 0u;
-                    if constexpr (RES) umma_ss_pair_pred(d, ka + 2 * k, qb + 2 * k, idesc, add, go);
-                    else umma_bf16_ss_pred(d, ka + 2 * k, qb + 2 * k, idesc, add, go);
+                    for (int k = 0; k < 4; ++k) {
+                        if (L::kBalanced && (k == 0 || k == 2) && half == k) multiply(d, ones, turn, 1u);
+                        multiply(d, ka + 2 * k, qb + 2 * k, L::kBalanced || s % L::kPerGroup || k ? 1u : 0u);
+                    }
                 }
                 commit(bars + (L::kBarEmpty + at) * 8);
                 if (RES && cb + 1 == cb1) commit(bars + (L::kBarKEmpty + s) * 8);
@@ -258,10 +288,11 @@ __device__ __forceinline__ void mma_role(const WeightsArgs &a, uint8_t *smem, ui
 }
 
 // ------------------------------------------------------------------ sums
-// Sum of exp2(s c - lse2) over `kCols` columns of this lane, each the sum of `groups` accumulators N columns apart; with MASK
-// only the columns in [lo, hi).
+// Sum of exp2((s + offset) c - lse2) over kCols columns of this lane, each the sum of `groups` accumulators N columns apart; with
+// MASK only the columns in [lo, hi).
 template <int kCols, int N, int kGroups, bool MASK>
-__device__ __forceinline__ void add_columns(uint32_t taddr, int groups, const float *lse2, float c, int lo, int hi, uint64_t (&acc)[4]) {
+__device__ __forceinline__ void add_columns(uint32_t taddr, int groups, const float *lse2, float c, float offset, int lo, int hi,
+                                            uint64_t (&acc)[4]) {
     uint32_t s[kCols];
     const auto load = [](uint32_t at, uint32_t (&r)[kCols]) {
         if constexpr (kCols == 32) {
@@ -281,13 +312,17 @@ __device__ __forceinline__ void add_columns(uint32_t taddr, int groups, const fl
             for (int j = 0; j < kCols; ++j) s[j] = __float_as_uint(__uint_as_float(s[j]) + __uint_as_float(x[j]));
         }
     }
-    const uint64_t c2 = pack2(c, c);
+    const uint64_t c2 = pack2(c, c), offset2 = pack2(offset, offset);
+    const auto score = [&](int j) {
+        const uint64_t v = pack2(__uint_as_float(s[j]), __uint_as_float(s[j + 1]));
+        return kGroups == 1 ? add2(v, offset2) : v;
+    };
 #pragma unroll
     for (int j = 0; j < kCols; j += 4) {
         const float4 z = *reinterpret_cast<const float4 *>(lse2 + j);    // negated
         float x[4];
-        unpack2(fma2(pack2(__uint_as_float(s[j]), __uint_as_float(s[j + 1])), c2, pack2(z.x, z.y)), x[0], x[1]);
-        unpack2(fma2(pack2(__uint_as_float(s[j + 2]), __uint_as_float(s[j + 3])), c2, pack2(z.z, z.w)), x[2], x[3]);
+        unpack2(fma2(score(j), c2, pack2(z.x, z.y)), x[0], x[1]);
+        unpack2(fma2(score(j + 2), c2, pack2(z.z, z.w)), x[2], x[3]);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             x[e] = fast_exp2(x[e]);
@@ -308,6 +343,7 @@ __device__ __forceinline__ void sum_role(const WeightsArgs &a, uint8_t *smem, ui
     float *sums = reinterpret_cast<float *>(smem + L::kSums);
     const uint32_t t_addr = tmem + group * N * L::kGroups + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const int blocks = RES ? (a.columns + N - 1) / N : 1, groups = (a.k_slabs + L::kPerGroup - 1) / L::kPerGroup;
+    const float offset = a.turn - a.start;       // exact
     uint32_t n_blocks = 0;
     bool failed = false;
     for (int it = 0;; ++it) {
@@ -345,17 +381,17 @@ __device__ __forceinline__ void sum_role(const WeightsArgs &a, uint8_t *smem, ui
             uint64_t acc[4] = {0, 0, 0, 0};
             if (from_warp <= c0 && c0 + N <= a.columns) {
 #pragma unroll 2
-                for (int j = 0; j < N; j += kCols) add_columns<kCols, N, L::kGroups, false>(t_addr + j, groups, lse2 + j, a.scale_log2, 0, 0, acc);
+                for (int j = 0; j < N; j += kCols) add_columns<kCols, N, L::kGroups, false>(t_addr + j, groups, lse2 + j, a.scale_log2, offset, 0, 0, acc);
             } else {
                 // columns of the block that count for this row (those past the last hold other queries' scores)
                 const int lo = from - c0, hi = a.columns - c0;
-                for (int j = 0; j < N; j += kCols) add_columns<kCols, N, L::kGroups, true>(t_addr + j, groups, lse2 + j, a.scale_log2, lo - j, hi - j, acc);
+                for (int j = 0; j < N; j += kCols) add_columns<kCols, N, L::kGroups, true>(t_addr + j, groups, lse2 + j, a.scale_log2, offset, lo - j, hi - j, acc);
             }
             tc_fence_before_sync();
             named_bar_sync(1 + group, 128);      // the scores and the lse buffer have been read
             if ((warp & 3) == 0 && lane == 0) {
                 const uint32_t s_free = bars + (L::kBarSFree + group) * 8;
-                if constexpr (RES) mbar_arrive_cluster(map_rank(s_free, 0));     // the even CTA issues for both
+                if constexpr (RES) mbar_arrive_remote(map_rank(s_free, 0));      // the even CTA issues for both
                 else mbar_arrive(s_free);
             }
             const uint64_t both = add2(add2(acc[0], acc[1]), add2(acc[2], acc[3]));
@@ -418,6 +454,12 @@ __global__ void __launch_bounds__(kThreads, 1) row_weights_kernel(const __grid_c
         }
         *abort_flag = 0;
         mbar_init_fence();
+    }
+    if constexpr (L::kBalanced) {
+        const uint32_t half = __float_as_uint(0.5f * a.start) >> 16, minus = __float_as_uint(-0.5f * a.turn) >> 16;   // exact in bf16
+        for (int x = L::kOnes + tid * 16; x < L::kLse; x += kThreads * 16)
+            *reinterpret_cast<uint4 *>(smem + x) = make_uint4(x < L::kStart ? 0x3F80u : x < L::kTurn ? half : minus, 0, 0, 0);
+        fence_async_smem();
     }
     if (warp == 8) {
         if constexpr (RES) tmem_alloc_pair(smem_u32(smem + L::kMisc + 8), L::kTmemCols);
@@ -529,6 +571,12 @@ int launch_row_weights(const smla_row_weights_params_t &p, int sm_count, cudaStr
     a.k_slabs = p.head_dim / 64;
     a.page = p.page_block_size;
     a.scale_log2 = p.softmax_scale * kLog2e;
+    const float range = 8.0f / std::fabs(p.softmax_scale);
+    if (range > 0.0f && range < INFINITY) {      // a scale of 0, or one as good as that, needs no offsets
+        const float base = std::ldexp(1.0f, std::min(100, std::max(-100, static_cast<int>(std::ceil(std::log2(range))))));
+        a.start = std::copysign(1.125f * base, p.softmax_scale);
+        a.turn = std::copysign(3.0f * base, p.softmax_scale);
+    }
     const int64_t rows = std::min<int64_t>(p.weights_width, static_cast<int64_t>(p.max_blocks_per_seq) * p.page_block_size);
     const int64_t tiles = std::max<int64_t>(1, (rows + 127) / 128) * p.batch;
     if (a.columns > 128) {
