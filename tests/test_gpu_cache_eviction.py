@@ -398,3 +398,138 @@ def test_prompt_decode_evict_decode(fm):
     before = acc.clone()
     fm.mla_cache_row_weights(q_abs, cache, table, kept, lse2, softmax_scale=scale, causal=True, weights=acc)
     assert ((acc - before).sum(1) - h).abs().max() < 1e-2 * h
+
+
+# ----------------------------------------------------------------------------- scales, plain C calls, several calls at once
+@pytest.mark.parametrize("scale", [-0.05, 0.0, 1e-30, 1e-3, 0.5])
+@pytest.mark.parametrize("s_q,h", [(1, 16), (1, 40), (1, 100), (3, 128)])
+def test_weights_scales(fm, s_q, h, scale):
+    kw, _ = paged([270, 65], s_q=s_q, h=h, seed=h)
+    lse = lse_of(kw, True, scale)
+    check_weights(fm.mla_cache_row_weights(**kw, softmax_lse=lse, softmax_scale=scale, causal=True), kw, lse, True, scale=scale)
+
+
+@pytest.mark.parametrize("s_q,h", [(1, 64), (1, 128), (2, 128), (9, 60)])
+def test_weights_of_rows_that_all_queries_look_at(fm, s_q, h):
+    # Scores up to about 10.  The rounding of the products' sums must not leave a bias: 38 steps that cut off up to one unit
+    # of 2^j 2^-23 (2^j times the scale <= 16) are 38^0.5 0.29 16 2^-23 = 3.4e-6 of one term where the steps' means cancel, but
+    # 38 / 2 x 16 x 2^-23 = 3.6e-5 where they do not; over the columns the former averages out, the latter does not.  Held to
+    # 2^-20 (3.4e-6 over 13 columns of equal weight; there are 64 and more) and 20 x 2^-22 for the exponents' rounding.
+    kw, _ = paged([500, 130], s_q=s_q, h=h, seed=3)
+    d = 576
+    u = torch.randn(d, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda")
+    kw["q"] = (kw["q"].float() * 0.6 + 0.6 * u).to(torch.bfloat16)
+    cache = kw["k_cache"].float()
+    cache[:, ::7] = cache[:, ::7] * 0.6 + 0.5 * u
+    kw["k_cache"] = cache.to(torch.bfloat16)
+    lse = lse_of(kw, False)
+    got = fm.mla_cache_row_weights(**kw, softmax_lse=lse).cpu().double()
+    ref, _ = oracle.cache_row_weights(kw["q"], kw["k_cache"], kw["block_table"], kw["cache_seqlens"], lse, width=got.shape[1])
+    for b, n in enumerate([500, 130]):
+        heavy = torch.zeros(got.shape[1], dtype=torch.bool)
+        heavy[:n] = ref[b, :n] > 0.2 * ref[b].max()
+        off = ((got - ref)[b, heavy] / ref[b, heavy])
+        assert heavy.sum() >= 10 and off.square().mean().sqrt() <= 2.0 ** -20 + 2.0 ** -22 * 20
+
+
+def _weights_params(abi, kw, lse, w, workspace=None, workspace_bytes=0, causal=1):
+    b, s_q, h, d = kw["q"].shape
+    k, t = kw["k_cache"], kw["block_table"]
+    return abi.SmlaRowWeightsParams(
+        batch=b, seqlen_q=s_q, num_heads=h, causal=causal, head_dim=d, softmax_scale=d ** -0.5, q=kw["q"].data_ptr(), softmax_lse=lse.data_ptr(),
+        k_cache=k.data_ptr(), k_block_stride=2 * k.stride(0), k_row_stride=2 * k.stride(1), num_blocks=k.shape[0], page_block_size=k.shape[1],
+        max_blocks_per_seq=t.shape[1], block_table=t.data_ptr(), block_table_stride=t.stride(0), cache_seqlens=kw["cache_seqlens"].data_ptr(),
+        weights=w.data_ptr(), weights_stride=w.stride(0), weights_width=w.shape[1], accumulate=0, workspace=workspace, workspace_bytes=workspace_bytes)
+
+
+@pytest.mark.parametrize("s_q,h", [(2, 128), (33, 20)])
+def test_weights_c_call_with_and_without_scratch(fm, s_q, h):
+    from flash_mla import c_abi
+    lib = c_abi.load()
+    kw, _ = paged([700, 1, 0, 513], s_q=s_q, h=h, seed=11)
+    lse = lse_of(kw, True)
+    need, none = ctypes.c_size_t(0), ctypes.c_size_t(1)
+    assert lib.smla_cache_row_weights_workspace(s_q, h, ctypes.byref(need)) == 0 and need.value > 0
+    assert lib.smla_cache_row_weights_workspace(1, 128, ctypes.byref(none)) == 0 and none.value == 0
+    scratch = torch.full((need.value + 16,), 255, dtype=torch.uint8, device="cuda")
+    stream = torch.cuda.current_stream().cuda_stream
+    for given in ((None, 0), (scratch.data_ptr(), need.value - 1), (scratch.data_ptr(), need.value)):
+        w = torch.full((4, kw["block_table"].shape[1] * 64), float("nan"), device="cuda")
+        assert lib.smla_cache_row_weights(ctypes.byref(_weights_params(c_abi, kw, lse, w, *given)), stream) == 0
+        check_weights(w, kw, lse, True, what=str(given))
+    assert (scratch[need.value:] == 255).all()
+    assert lib.smla_cache_row_weights(ctypes.byref(_weights_params(c_abi, kw, lse, w, scratch.data_ptr() + 4, need.value)), stream) == -2
+
+
+def test_calls_on_several_streams_at_once(fm):
+    calls = []
+    for i, (s_q, h) in enumerate([(1, 16), (4, 128), (1, 64), (16, 32)]):
+        kw, _ = paged([3000, 77, 1500], s_q=s_q, h=h, seed=20 + i)
+        lse = torch.full((3, h, s_q), 7.5, device="cuda")
+
+        def run(kw=kw, lse=lse):
+            w = fm.mla_cache_row_weights(**kw, softmax_lse=lse, causal=True)
+            rows, kept, sums = fm.mla_select_cache_rows(w, kw["cache_seqlens"], 600, 50)
+            cache = kw["k_cache"].clone()
+            fm.mla_compact_cache(cache, kw["block_table"], rows, kept)
+            return w, rows, kept, sums, cache.view(torch.int16)
+        calls.append(run)
+    want = [run() for run in calls]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in calls]
+    got = []
+    for _ in range(3):
+        for run, s in zip(calls, streams):
+            with torch.cuda.stream(s):
+                got.append(run())
+    torch.cuda.synchronize()
+    for i, out in enumerate(got):
+        for a, b in zip(out, want[i % len(calls)]):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("in_place", [True, False])
+def test_eviction_in_a_graph(fm, in_place):
+    lens, budget = [400, 90, 260], 100
+    kw, spare = paged(lens, s_q=2, h=128, seed=31, extra=0 if in_place else 6)
+    out = None if in_place else spare.view(3, 2).cuda()
+    start = kw["k_cache"].clone()
+    lse = lse_of(kw, True)
+
+    def step():
+        w = fm.mla_cache_row_weights(**kw, softmax_lse=lse, causal=True)
+        rows, kept, sums = fm.mla_select_cache_rows(w, kw["cache_seqlens"], budget, 30)
+        fm.mla_compact_cache(kw["k_cache"], kw["block_table"], rows, kept, out_block_table=out)
+        return rows, kept, sums
+    want = [x.clone() for x in step()]
+    moved = kw["k_cache"].clone()
+    assert same_bytes(moved, oracle.compact_cache(start, kw["block_table"], want[0], want[1], out))
+    torch.cuda.synchronize()
+    kw["k_cache"].copy_(start)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for _ in range(2):
+        kw["k_cache"].copy_(start)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+        assert same_bytes(kw["k_cache"], moved)
+
+
+def test_pages_far_into_a_large_cache(fm):
+    # element offsets past 2^31: 65600 pages of 64 rows (4.8 GB), of which the last hold the sequences
+    nb, lens = 65600, [200, 70]
+    kw, _ = paged(lens, h=16, seed=41)
+    small, table = kw["k_cache"], kw["block_table"]
+    big = torch.empty(nb, 64, 1, 576, dtype=torch.bfloat16, device="cuda")
+    big[nb - small.shape[0]:] = small
+    far = torch.where(table >= 0, table + (nb - small.shape[0]), table)
+    lse = lse_of(kw, True)
+    w = fm.mla_cache_row_weights(kw["q"], big, far, kw["cache_seqlens"], lse, causal=True)
+    check_weights(w, kw, lse, True)
+    rows, kept, _ = fm.mla_select_cache_rows(w, kw["cache_seqlens"], 64, 10)
+    want = oracle.compact_cache(small, table, rows, kept)
+    fm.mla_compact_cache(big, far, rows, kept)
+    assert same_bytes(big[nb - small.shape[0]:], want)

@@ -245,3 +245,15 @@ def test_random_shapes(fm):
         a = inputs(ql, kl, h=hk * rng.choice([1, 2, 3]), hk=hk, d=rng.choice([128, 192]), dt=rng.choice([torch.bfloat16, torch.float16]), seed=i)
         causal = rng.random() < 0.7
         check(fm.dense_mla_prefill(*a, causal=causal), a, causal=causal, what=f"{i}: {ql} {kl} causal={causal}")
+
+
+def test_offsets_past_2_31_elements(fm):
+    # 66000 tokens of 256 x 192 (6.5 GB) and 256 x 128 elements; the only sequence lies at the end
+    n, h, m = 66000, 256, 150
+    a = inputs([m], h=h, hk=2, seed=16)
+    q = torch.empty(n, h, 192, dtype=torch.bfloat16, device="cuda")
+    q[n - m:] = a[0]
+    k, v = (torch.cat([torch.full((n - m,) + x.shape[1:], float("nan"), dtype=x.dtype, device="cuda"), x]) for x in a[1:3])
+    at = torch.tensor([n - m, n], dtype=torch.int32, device="cuda")
+    out, lse = fm.dense_mla_prefill(q, k, v, at, at)
+    check((out[n - m:], lse[:, n - m:]), a)
