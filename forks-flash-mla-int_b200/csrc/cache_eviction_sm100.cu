@@ -8,14 +8,17 @@
 // Counts are integers, so nothing depends on the order of the atomics.
 //
 // A cluster of CTAs takes a sequence.  Each holds its part of the keys in shared memory, so the weights are read
-// once, and the counts of a pass are added up through distributed shared memory.  What bounds it is latency: the four
-// passes, each a count, a cluster barrier and a search, one after the other.
+// once, and the counts of a pass are added up through distributed shared memory.  What bounds it is latency: the
+// passes (two to four), each a count, a cluster barrier and a search, one after the other.  64 sequences of 32768 rows, two
+// CTAs each: 19 us, of which reading the weights (8 MB) would be 1.3; of 15 in the kernel the first pass takes 4, the second 3,
+// counting what stays 1.6 and writing it 4.5.  Four sequences of 2048 rows: 8 us back to back, 4 of them in the kernel.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 #include <algorithm>
 #include <cstdint>
 
 #include "smla_internal.h"
+#include "tensor_map.h"
 
 namespace smla {
 namespace {
@@ -31,6 +34,8 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
     const uint32_t u = __float_as_uint(w + 0.0f);            // -0 + 0 = 0
     return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
+// The weight of a key that is neither a zero's nor a NaN's.
+__device__ __forceinline__ float key_weight(uint32_t k) { return __uint_as_float((k & 0x80000000u) ? k ^ 0x80000000u : ~k); }
 
 __global__ void __launch_bounds__(kSelThreads, 1) select_rows_kernel(const float *weights, int64_t stride, int width, const int32_t *lens,
                                                                      int budget, int recent, int held, int32_t *rows, int32_t *kept,
@@ -135,40 +140,24 @@ __global__ void __launch_bounds__(kSelThreads, 1) select_rows_kernel(const float
         want = static_cast<unsigned>(s_left);
         if (shift == 0 || s_all) break;
     }
-    // Rows whose key, without the bits not looked at, is above the prefix stay, and the first `want` that equal it.  A warp
-    // takes consecutive rows, a lane four of them at a time.
+    // Rows whose key, without the bits not looked at, is above the prefix stay, and the first `want` that equal it: keys above
+    // `high`, and those from `low` on.  A warp takes consecutive rows.
+    const uint32_t low = prefix << shift, high = low | ((1u << shift) - 1u);
     const int warp_part = ((n + kSelWarps - 1) / kSelWarps + 127) & ~127;
-    const int w_lo = min(warp * warp_part, n), w_hi = min(w_lo + warp_part, n);
-    const auto four = [&](int j, uint32_t (&k)[4]) {         // keys of rows j .. j + 3, shifted, and which of them there are
-        if (j + 3 < min(n, held)) {
-            const uint4 x = *reinterpret_cast<const uint4 *>(keys + j);
-            k[0] = x.x >> shift;
-            k[1] = x.y >> shift;
-            k[2] = x.z >> shift;
-            k[3] = x.w >> shift;
-            return 0xFu;
-        }
-        unsigned have = 0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            k[e] = 0;
-            if (j + e < n) {
-                k[e] = key_at(j + e) >> shift;
-                have |= 1u << e;
-            }
-        }
-        return have;
-    };
+    const int w_lo = min(warp * warp_part, n), w_hi = min(w_lo + warp_part, n), w_held = min(w_hi, held);
     int above = 0, equal = 0;
-    for (int j = w_lo + lane * 4; j < w_hi; j += 128) {
-        uint32_t k[4];
-        const unsigned have = four(j, k);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            above += ((have >> e) & 1u) && k[e] > prefix;
-            equal += ((have >> e) & 1u) && k[e] == prefix;
-        }
+    int j_rest = w_lo;
+    for (; j_rest + 128 <= w_held; j_rest += 128) {
+        const uint4 k = *reinterpret_cast<const uint4 *>(keys + j_rest + lane * 4);
+        above += (k.x > high) + (k.y > high) + (k.z > high) + (k.w > high);
+        equal += (k.x >= low) + (k.y >= low) + (k.z >= low) + (k.w >= low);
     }
+    for (int j = j_rest + lane; j < w_hi; j += 32) {
+        const uint32_t k = key_at(j);
+        above += k > high;
+        equal += k >= low;
+    }
+    equal -= above;
     above = __reduce_add_sync(0xffffffffu, above);
     equal = __reduce_add_sync(0xffffffffu, equal);
     if (lane == 0) {
@@ -203,42 +192,35 @@ __global__ void __launch_bounds__(kSelThreads, 1) select_rows_kernel(const float
         equal += *cluster.map_shared_rank(&s_sum[1], r);
     }
     const int ties = static_cast<int>(want);
+    const unsigned before = (1u << lane) - 1u;
     for (int j0 = w_lo; j0 < w_hi; j0 += 128) {
-        const int j = j0 + lane * 4;
         uint32_t k[4];
-        const unsigned have = four(j, k);
-        unsigned is_above = 0, is_equal = 0;
+        unsigned up[4], tie[4];                  // lanes with a row above, equal
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            is_above |= static_cast<unsigned>(k[e] > prefix) << e;
-            is_equal |= static_cast<unsigned>(k[e] == prefix) << e;
+            const int j = j0 + e * 32 + lane;
+            const bool there = j < w_hi;
+            k[e] = j < w_held ? keys[j] : there ? key_at(j) : 0u;
+            up[e] = __ballot_sync(0xffffffffu, k[e] > high);
+            tie[e] = __ballot_sync(0xffffffffu, there && k[e] >= low) & ~up[e];
         }
-        is_above &= have;
-        is_equal &= have;
-        const int both = __popc(is_above) | (__popc(is_equal) << 16);
-        int upto = both;
 #pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const int x = __shfl_up_sync(0xffffffffu, upto, d);
-            if (lane >= d) upto += x;
-        }
-        const int sum = __shfl_sync(0xffffffffu, upto, 31), front = upto - both;
-        int a = above + (front & 0xFFFF), t = equal + (front >> 16);
-        if (is_above | is_equal) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const bool up = (is_above >> e) & 1u, tie = (is_equal >> e) & 1u;
-                if (up || (tie && t < ties)) {
-                    const int at = a + min(t, ties);
-                    rows[at] = lo + j + e;
-                    if (kept_weights) kept_weights[at] = __ldg(mine + j + e);
-                }
-                a += up;
-                t += tie;
+        for (int e = 0; e < 4; ++e) {
+            int t = equal;
+            bool stays = k[e] > high;
+            if (tie[e]) {
+                t += __popc(tie[e] & before);
+                stays |= ((tie[e] >> lane) & 1u) && t < ties;
+                equal += __popc(tie[e]);
             }
+            if (stays) {
+                const int at = above + __popc(up[e] & before) + min(t, ties), j = j0 + e * 32 + lane;
+                rows[at] = lo + j;
+                // out of the key: reading it again costs the latency of memory
+                if (kept_weights) kept_weights[at] = k[e] == 0u || k[e] == 0x80000000u ? __ldg(mine + j) : key_weight(k[e]);
+            }
+            above += __popc(up[e]);
         }
-        above += sum & 0xFFFF;
-        equal += sum >> 16;
     }
     for (int j = all; j < recent; j += step) {
         rows[want0 + j] = old + j;
@@ -337,8 +319,10 @@ int launch_select_rows(const float *weights, int64_t weights_stride, int width, 
     while (ranks < 8 && width / ranks > kMaxKeys) ranks *= 2;
     const int part = ((width + ranks - 1) / ranks + 31) & ~31, held = std::min(part, kMaxKeys);
     if (static_cast<int64_t>(batch) * ranks > 0x7FFFFFFFLL) return SMLA_ETOOBIG;
-    cudaError_t e = cudaFuncSetAttribute(select_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxKeys * 4);
-    if (e != cudaSuccess) return static_cast<int>(e);
+    static KernelSetup setup;
+    int *status;                                 // (this kernel waits for nothing that could fail to come)
+    const int rc = setup.get(reinterpret_cast<const void *>(&select_rows_kernel), kMaxKeys * 4, &status);
+    if (rc != 0) return rc;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(batch) * ranks);
     cfg.blockDim = dim3(kSelThreads);
@@ -350,8 +334,7 @@ int launch_select_rows(const float *weights, int64_t weights_stride, int width, 
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, select_rows_kernel, weights, weights_stride, width, lens, budget, recent, held, rows, kept, kept_weights);
-    return static_cast<int>(e);
+    return static_cast<int>(cudaLaunchKernelEx(&cfg, select_rows_kernel, weights, weights_stride, width, lens, budget, recent, held, rows, kept, kept_weights));
 }
 
 int launch_compact(const smla_compact_params_t &p, int, cudaStream_t stream) {
