@@ -1,7 +1,7 @@
 """Eviction of rows from the paged bf16 cache of dense MLA decode, by the attention they got.
 
-A cached latent row that hardly any query looks at can go when the pool is full.  Three calls, each one kernel,
-none of which synchronises:
+A cached latent row that hardly any query looks at can go when the pool is full.  Three calls, each one kernel (the
+weights of a window two), none of which synchronises:
 
 ``mla_cache_row_weights``   adds up, for every cached row, the attention weight that the queries of a
                             ``flash_mla_with_kvcache`` call gave it, from the log-sum-exp that call returned;

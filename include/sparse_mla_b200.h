@@ -232,8 +232,9 @@ SMLA_API int smla_dense_mla_prefill(const smla_prefill_params_t *params, void *s
  *      w[b, r] = sum over i, h with r visible to query i of exp(scale q[b, i, h, :] . K[b, r, :] - lse[b, h, i]).
  *    `accumulate` adds it to what `weights` holds for the rows of the sequence and leaves the others as they are;
  *    without it the whole [batch, weights_width] is written, 0 behind the sequence's rows.  A query whose lse is
- *    -inf gives nothing.  Sums are fp32 in a fixed order (two calls give the same bits).  A page number outside
- *    the cache is a page of zero rows, as in the decode. */
+ *    -inf gives nothing.  Sums are fp32 in a fixed order (two calls give the same bits; another workspace, another GPU
+ *    or other sequences beside a sequence may change the order).  A page number outside the cache is a page of zero
+ *    rows, as in the decode.  One launch, with a workspace two. */
 typedef struct smla_row_weights_params {
     int32_t batch, seqlen_q, num_heads;   /* q [batch, seqlen_q, num_heads, head_dim] bf16                       */
     int32_t causal;                       /* query position i sees the first len - (seqlen_q - 1 - i) rows       */
@@ -255,7 +256,7 @@ typedef struct smla_row_weights_params {
     int32_t accumulate;
     void *workspace;                      /* 16-byte aligned scratch of smla_cache_row_weights_workspace bytes, which lets
                                              windows of more than 128 (position, head) pairs use every SM; NULL or less:
-                                             whole tiles of 128 rows are dealt out.  Calls that overlap on the GPU need
+                                             whole tiles of 256 rows are dealt out.  Calls that overlap on the GPU need
                                              one each                                                             */
     size_t workspace_bytes;
 } smla_row_weights_params_t;
