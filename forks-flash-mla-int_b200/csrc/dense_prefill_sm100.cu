@@ -122,7 +122,8 @@ __device__ __forceinline__ Seq seq_of(const PrefillArgs &a, int b) {
 
 struct Walk {                                    // uniform over the loader warp
     int high, shift;                             // highest level of the bucket
-    long long base;                              // items in the buckets above
+    int b0;                                      // first of the 32 sequences looked at
+    long long base;                              // items in front of theirs
 };
 // Items (per head) of sequence s in a bucket.
 __device__ __forceinline__ int in_bucket(const Seq &s, const Walk &w) {
@@ -138,19 +139,17 @@ __device__ __forceinline__ void start_walk(const PrefillArgs &a, Walk &w, int la
     w.high = __reduce_max_sync(0xffffffffu, top);
     w.shift = 1;
     while ((w.high >> w.shift) >= 32) ++w.shift;
+    w.b0 = 0;
     w.base = 0;
 }
 // Item `idx` (not below any asked for before) as a record; false behind the last.
 __device__ __forceinline__ bool find_item(const PrefillArgs &a, Walk &w, long long idx, int lane, int *rec) {
-    for (; w.high > 0; w.high -= 1 << w.shift) {
-        int r = -1;                              // rank of the item among those of the bucket, without the head
-        if (idx >= w.base) r = static_cast<int>(min((idx - w.base) / a.heads, 0x7FFFFFFFll));
-        int before = 0;
-        for (int b0 = 0; b0 < a.batch; b0 += 32) {
+    for (; w.high > 0; w.high -= 1 << w.shift, w.b0 = 0) {
+        for (; w.b0 < a.batch; w.b0 += 32) {
             Seq s = {};
             int n = 0;
-            if (b0 + lane < a.batch) {
-                s = seq_of(a, b0 + lane);
+            if (w.b0 + lane < a.batch) {
+                s = seq_of(a, w.b0 + lane);
                 n = s.blocks > 0 ? in_bucket(s, w) : 0;
             }
             int upto = n;                        // inclusive prefix sum over the lanes
@@ -159,18 +158,16 @@ __device__ __forceinline__ bool find_item(const PrefillArgs &a, Walk &w, long lo
                 const int x = __shfl_up_sync(0xffffffffu, upto, d);
                 if (lane >= d) upto += x;
             }
-            const unsigned hit = __ballot_sync(0xffffffffu, r >= before + upto - n && r < before + upto);
-            if (hit != 0u) {
-                const int src = __ffs(hit) - 1;
+            const long long here = static_cast<long long>(__shfl_sync(0xffffffffu, upto, 31)) * a.heads;
+            if (idx < w.base + here) {
                 // head after head, whose items are neighbours (they read the same keys); levels fall, from the highest that the
                 // sequence has in the bucket
-                const long long local = (idx - w.base) - static_cast<long long>(before + upto - n) * a.heads;
-                const int of = max(n, 1), head = static_cast<int>(local / of);
-                const int level = min(w.high, s.top) - static_cast<int>(local % of);
-                const int m0 = (s.blocks - 1 - (s.top - level)) << 8;
-                const int rows = min(256, s.nq - m0), off = m0 + s.nk - s.nq;
-                const int see = a.causal ? min(s.nk, max(0, off + rows)) : s.nk;         // keys that the item's last row sees
-                if (lane == src) {
+                const long long local = idx - w.base - static_cast<long long>(upto - n) * a.heads;
+                if (local >= 0 && local < static_cast<long long>(n) * a.heads) {         // one lane
+                    const int head = static_cast<int>(local / n), level = min(w.high, s.top) - static_cast<int>(local % n);
+                    const int m0 = (s.blocks - 1 - (s.top - level)) << 8;
+                    const int rows = min(256, s.nq - m0), off = m0 + s.nk - s.nq;
+                    const int see = a.causal ? min(s.nk, max(0, off + rows)) : s.nk;     // keys that the item's last row sees
                     rec[kRecValid] = 1;
                     rec[kRecQRow] = s.q0 + m0;
                     rec[kRecRows] = rows;
@@ -182,9 +179,8 @@ __device__ __forceinline__ bool find_item(const PrefillArgs &a, Walk &w, long lo
                 }
                 return true;
             }
-            before += __shfl_sync(0xffffffffu, upto, 31);
+            w.base += here;
         }
-        w.base += static_cast<long long>(before) * a.heads;
     }
     return false;
 }

@@ -257,3 +257,12 @@ def test_offsets_past_2_31_elements(fm):
     at = torch.tensor([n - m, n], dtype=torch.int32, device="cuda")
     out, lse = fm.dense_mla_prefill(q, k, v, at, at)
     check((out[n - m:], lse[:, n - m:]), a)
+
+
+def test_many_prompts_of_mixed_lengths(fm):
+    import random
+    rng = random.Random(17)
+    ql = [rng.choice([0, 1, 2, 30, 130, 257, 600]) for _ in range(75)]
+    kl = [x + rng.choice([0, 0, 1, 200, 700]) for x in ql]
+    a = inputs(ql, kl, h=3, seed=18)
+    check(fm.dense_mla_prefill(*a), a)
