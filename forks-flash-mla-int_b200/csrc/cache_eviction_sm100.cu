@@ -300,7 +300,7 @@ __global__ void __launch_bounds__(kSliceThreads) move_rows_in_place_kernel(const
         for (int e = 0; e < kTurnPieces; ++e) {
             const int j = j0 + e * (kTurnRows / kTurnPieces) + threadIdx.x / (kSlice / 16);
             if (j < n && at < p.row_bytes) {
-                uint8_t *dst = const_cast<uint8_t *>(row_at(p, table, p.max_blocks_per_seq, j));
+                uint8_t *dst = const_cast<uint8_t *>(row_at(p, table, p.out_max_blocks_per_seq, j));
                 if (dst) *reinterpret_cast<uint4 *>(dst + at) = x[e];
             }
         }
@@ -339,7 +339,7 @@ int launch_select_rows(const float *weights, int64_t weights_stride, int width, 
 
 int launch_compact(const smla_compact_params_t &p, int, cudaStream_t stream) {
     if (p.batch > 65535) return SMLA_ETOOBIG;
-    if (p.out_block_table == p.block_table) {
+    if (p.out_block_table == p.block_table && (p.batch <= 1 || p.out_block_table_stride == p.block_table_stride)) {
         move_rows_in_place_kernel<<<dim3(static_cast<unsigned>((p.row_bytes + kSlice - 1) / kSlice), static_cast<unsigned>(p.batch)), kSliceThreads, 0, stream>>>(p);
     } else {
         constexpr int per_block = kMoveWarps * kMoveRows;

@@ -587,11 +587,12 @@ void mla_compact_cache(const Tensor &cache, const Tensor &table_in, const Tensor
     if (out_table_in.has_value()) check_paged(cache, out_table_in.value(), device, B, what);
     torch::stable::accelerator::DeviceGuard guard(device);
     const Tensor table = as_table(table_in);
-    // the caller's own table given as the target means a move in place, also where a copy of it had to be made
+    // the caller's own table (or its first columns) given as the target means a move in place, also where a copy of it had to
+    // be made
     const bool in_place = !out_table_in.has_value() ||
-                          (out_table_in->data_ptr() == table_in.data_ptr() && out_table_in->size(1) == table_in.size(1) &&
+                          (out_table_in->data_ptr() == table_in.data_ptr() && out_table_in->size(1) <= table_in.size(1) &&
                            (B <= 1 || out_table_in->stride(0) == table_in.stride(0)) &&
-                           (table_in.size(1) <= 1 || out_table_in->stride(1) == table_in.stride(1)));
+                           (out_table_in->size(1) <= 1 || out_table_in->stride(1) == table_in.stride(1)));
     const Tensor out_table = in_place ? table : as_table(out_table_in.value());
     const Tensor rows = rows_in.is_contiguous() ? rows_in : torch::stable::contiguous(rows_in);
     const Tensor kept = kept_in.is_contiguous() ? kept_in : torch::stable::contiguous(kept_in);
@@ -609,7 +610,7 @@ void mla_compact_cache(const Tensor &cache, const Tensor &table_in, const Tensor
     p.max_blocks_per_seq = static_cast<int32_t>(table.size(1));
     p.out_block_table = static_cast<const int32_t *>(out_table.data_ptr());
     p.out_block_table_stride = row_stride_2d(out_table);
-    p.out_max_blocks_per_seq = static_cast<int32_t>(out_table.size(1));
+    p.out_max_blocks_per_seq = static_cast<int32_t>(out_table_in.has_value() ? out_table_in->size(1) : table.size(1));
     p.rows = static_cast<const int32_t *>(rows.data_ptr());
     p.kept = static_cast<const int32_t *>(kept.data_ptr());
     check_rc(smla_compact_cache(&p, current_stream(device)), what);

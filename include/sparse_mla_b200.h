@@ -274,8 +274,9 @@ SMLA_API int smla_select_cache_rows(const float *weights, int64_t weights_stride
                                     int32_t *kept, float *kept_weights, void *stream);
 
 /* 3. smla_compact_cache: row rows[b, j] of sequence b (through block_table) becomes its row j (through
- *    out_block_table), j < kept[b].  rows [batch, budget] contiguous.  With out_block_table == block_table the rows
- *    move inside their own pages: rows must then ascend, with rows[b, j] >= j (as selected above).  Otherwise the
+ *    out_block_table), j < kept[b].  rows [batch, budget] contiguous.  With out_block_table == block_table and
+ *    the same stride the rows move inside their own pages: rows must then ascend, with rows[b, j] >= j (as
+ *    selected above).  Otherwise the
  *    pages written must not be among the pages read.  In both cases no page may be written for two sequences (or
  *    twice for one).  A source row outside the table or the cache is a zero row; a target outside is left out.
  *    row_bytes, strides and base are multiples of 16. */

@@ -533,3 +533,59 @@ def test_pages_far_into_a_large_cache(fm):
     want = oracle.compact_cache(small, table, rows, kept)
     fm.mla_compact_cache(big, far, rows, kept)
     assert same_bytes(big[nb - small.shape[0]:], want)
+
+
+@pytest.mark.parametrize("copied", [False, True])
+def test_compact_into_the_first_pages_of_the_table(fm, copied):
+    lens, budget = [700, 300, 90], 200
+    kw, _ = paged(lens, h=1, d=64, page=16, seed=51)
+    rows, kept = ascending(lens, budget, 7)
+    table = kw["block_table"]
+    if copied:                                                # a strided table that the binding has to copy
+        table = torch.stack([table, table], 2)[:, :, 0]
+    want = oracle.compact_cache(kw["k_cache"], table, rows, kept, table[:, :5])
+    fm.mla_compact_cache(kw["k_cache"], table, rows, kept, out_block_table=table[:, :5])
+    assert same_bytes(kw["k_cache"], want)
+
+
+_FIRST_CALL = """
+import torch, flash_mla as fm
+dev = "cuda"
+g = torch.Generator(device=dev).manual_seed(0)
+q = torch.randn(1, 2, 128, 576, generator=g, device=dev).to(torch.bfloat16)
+cache = torch.randn(8, 64, 1, 576, generator=g, device=dev).to(torch.bfloat16)
+table = torch.arange(8, dtype=torch.int32, device=dev)[None]
+lens = torch.full((1,), 500, dtype=torch.int32, device=dev)
+lse = torch.full((1, 128, 2), 7.0, device=dev)
+p = torch.randn(300, 4, 192, generator=g, device=dev).to(torch.bfloat16)
+v = torch.randn(300, 4, 128, generator=g, device=dev).to(torch.bfloat16)
+cu = torch.tensor([0, 300], dtype=torch.int32, device=dev)
+
+def step():
+    w = fm.mla_cache_row_weights(q, cache, table, lens, lse)
+    w1 = fm.mla_cache_row_weights(q[:, :1, :16].contiguous(), cache, table, lens, lse[:, :16, :1].contiguous())
+    rows, kept, sums = fm.mla_select_cache_rows(w, lens, 100, 10)
+    moved = cache.clone()
+    fm.mla_compact_cache(moved, table, rows, kept)
+    out, z = fm.dense_mla_prefill(p, p, v, cu, cu)
+    return w, w1, rows, kept, sums, moved.view(torch.int16), out, z
+
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = step()
+graph.replay()
+torch.cuda.synchronize()
+for a, b in zip(got, step()):
+    assert torch.equal(a, b)
+print("captured", fm.__name__)
+"""
+
+
+def test_the_first_call_of_a_process_may_be_a_captured_one(fm):
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(fm.__file__)))
+    run = subprocess.run([sys.executable, "-c", _FIRST_CALL], env={**os.environ, "PYTHONPATH": root}, capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and "captured" in run.stdout, run.stderr[-2000:]
