@@ -89,7 +89,8 @@ struct Smem {
     static constexpr int kQueue = kSums + 128 * 8;                       // eight items {blocks, keys} with scores not yet added
     static constexpr int kTurn = kQueue + 8 * 8;                         // [kRecords][4] whether the warps of a quarter go on
     static constexpr int kMisc = kTurn + kRecords * 4 * 4;               // abort flag, tensor memory address
-    static constexpr int kBytes = kMisc + 16;
+    static constexpr int kOut = (kMisc + 16 + 127) & ~127;               // [4][32 rows][32 columns] of output on their way
+    static constexpr int kBytes = kOut + 4 * 2048;
 };
 static_assert(Smem<192>::kBytes <= 232448 && Smem<128>::kBytes <= 232448, "shared memory of one CTA");
 
@@ -492,8 +493,12 @@ __device__ __forceinline__ void softmax_role(const PrefillArgs &a, uint8_t *smem
             if (t * 128 + 128 > lim_warp) {
                 const int see = lim - t * 128;
 #pragma unroll
-                for (int j = 0; j < 128; ++j)
-                    if (j >= see) s[j] = 0xFF800000u;
+                for (int j = 0; j < 128; j += 32) {
+                    const uint32_t hidden = see >= j + 32 ? 0u : see <= j ? ~0u : ~0u << (see - j);
+#pragma unroll
+                    for (int e = 0; e < 32; ++e)
+                        if ((hidden >> e) & 1u) s[j + e] = 0xFF800000u;
+                }
             }
             float mx[4];
 #pragma unroll
@@ -577,35 +582,44 @@ __device__ __forceinline__ void softmax_role(const PrefillArgs &a, uint8_t *smem
         }
         const float top = fmaxf(m, other.x);
         const float l = top == -INFINITY ? mine_l + other.y : mine_l * fast_exp2(m - top) + other.y * fast_exp2(other.x - top);    // 0, or NaN from NaN
-        const bool mine = row < rows;
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        if (mine && a.lse != nullptr) a.lse[head * a.lse_hs + qrow + row] = l == 0.0f ? -INFINITY : (top + log2f(l)) * kLn2;
-        uint16_t *dst = static_cast<uint16_t *>(a.out) + (qrow + row) * a.o_ts + head * a.o_hs;
+        if (row < rows && a.lse != nullptr) a.lse[head * a.lse_hs + qrow + row] = l == 0.0f ? -INFINITY : (top + log2f(l)) * kLn2;
         if (n > 0) {
             failed |= !mbar_wait(bars + L::kBarO * 8, n_items & 1, abort_flag);
             tc_fence_after_sync();
         }
-#pragma unroll
+        // A warp's rows go through shared memory 32 columns at a time, so that four lanes store 64 consecutive bytes: 16 bytes of
+        // each row at a time, straight from the lanes, take 32 cycles of the load and store unit per instruction.
+        uint8_t *stage = smem + L::kOut + quarter * 2048;
+        const int first = rank * 128 + quarter * 32 + (lane >> 2);
+        uint16_t *dst = static_cast<uint16_t *>(a.out) + (qrow + first) * a.o_ts + head * a.o_hs + (lane & 3) * 8;
+        const bool store = !__any_sync(0xffffffffu, failed);
+#pragma unroll 1
         for (int j = 0; j < 128; j += 32) {
-            uint32_t o[32];
+            uint4 w[4] = {};
             if (n > 0) {
+                uint32_t o[32];
                 tmem_ld_x32_nowait(o_addr + j, o);
                 tmem_ld_wait();
-                if (j == 96) {
-                    tc_fence_before_sync();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(bars + (L::kBarRead + quarter) * 8);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    uint32_t x[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)      // a row without keys: zeros (the accumulator may hold anything)
+                        x[i] = l == 0.0f ? 0u : pack16<FP16>(__uint_as_float(o[e * 8 + 2 * i]) * inv, __uint_as_float(o[e * 8 + 2 * i + 1]) * inv);
+                    *reinterpret_cast<uint4 *>(stage + lane * 64 + ((e ^ (lane >> 1)) & 3) * 16) = make_uint4(x[0], x[1], x[2], x[3]);
                 }
+                __syncwarp();
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[e] = *reinterpret_cast<const uint4 *>(stage + e * 512 + (lane >> 2) * 64 + ((lane ^ (lane >> 3)) & 3) * 16);
+                tc_fence_before_sync();
+                __syncwarp();
+                if (j == 96 && lane == 0) mbar_arrive(bars + (L::kBarRead + quarter) * 8);
             }
-            if (mine && !failed) {
+            if (store) {
 #pragma unroll
-                for (int e = 0; e < 32; e += 8) {
-                    uint32_t w[4];
-#pragma unroll
-                    for (int x = 0; x < 4; ++x)      // a row without keys: zeros (the accumulator may hold anything)
-                        w[x] = l == 0.0f ? 0u : pack16<FP16>(__uint_as_float(o[e + 2 * x]) * inv, __uint_as_float(o[e + 2 * x + 1]) * inv);
-                    *reinterpret_cast<uint4 *>(dst + j + e) = make_uint4(w[0], w[1], w[2], w[3]);
-                }
+                for (int e = 0; e < 4; ++e)
+                    if (first + e * 8 < rows) *reinterpret_cast<uint4 *>(dst + e * 8 * a.o_ts + j) = w[e];
             }
         }
         if (n > 0) ++n_items;
