@@ -18,18 +18,20 @@
 // Three tiles are scored ahead of the output, so the weights of a tile have the time of two tiles' products to be computed
 // in, and two warpgroups take turns at the tiles: a weight computation (about 2100 cycles for a tile, one row per thread)
 // may take nearly twice as long as the products of a tile (1280 cycles at 192 dims).
-// What bounds it: tensor work, at 88 % while a long item runs (1460 cycles a tile: the chain weights - output - score of the
-// tile three on takes a little longer than three tiles' products).  8192 causal tokens of 37 heads: 594 us with 192 dims
-// (1.34 PFLOP/s), 529 us with 128 (1.20).  Measured against it: one CTA per item, S in one buffer for each half of the rows,
-// 675 and 580 us; weights in buffers of their own beside S (a fourth wait and narrower stores) 660 and 587; weights handed
-// over in two pieces 602 and 530; the rows' reference through mbarriers in place of named ones 600 and 542.
+// What bounds it: tensor work, at 88 % while a long item runs (1400 cycles a tile: the chain weights - output - score of the
+// tile three on takes a little longer than three tiles' products), and the power limit in long runs.  From item to item the
+// output takes about 4000 cycles (last product, read, first product), of which half is hidden.  8192 causal tokens of 37
+// heads: 573 us with 192 dims (1.39 PFLOP/s), 502 us with 128 (1.27).  Measured against it: one CTA per item, S in one buffer
+// for each half of the rows, 675 and 580 us; weights in buffers of their own beside S (a fourth wait and narrower stores)
+// 660 and 587; weights handed over in two pieces 602 and 530; the rows' reference through mbarriers in place of named ones
+// 600 and 542; the output written by the softmax warpgroup that had the last tile 577 and 509.
 // K and V arrive by TMA as slabs of 64 dims with the 128-byte swizzle: of K the rows of 64 keys (its half of N), of V all
 // 128 keys of 64 of the dims (its half of N there).  A slab read K-major gives K for the first product, MN-major V for the
 // second.  Sharing B halves the fills: with both operands from shared memory one CTA's products alone (M = N = 128) take all
 // of its 128 bytes a cycle.
 //
-// Roles (384 threads): warps 0-3 and 4-7 are the two softmax warpgroups, warp 8 (of the even CTA) issues the products, warp 9
-// finds the items and loads Q and K, warp 10 loads V.  Item records go through a ring of four in shared memory.
+// Roles (512 threads): warps 0-3 and 4-7 are the two softmax warpgroups, warp 8 (of the even CTA) issues the products, warp 9
+// finds the items and loads Q and K, warp 10 loads V, warps 12-15 write the output.  Item records go through a ring of four in shared memory.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -46,16 +48,16 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr int kThreads = 384;
+constexpr int kThreads = 512;
 constexpr int kSlab = 128 * 128;                 // bytes of [128 rows][64 dims] of 16-bit elements
 constexpr int kHalfSlab = kSlab / 2;             // [64 rows][64 dims]
 constexpr int kRecords = 4;
 constexpr int kRecInts = 12;
 constexpr int kBuffers = 3;                      // of S
 constexpr uint32_t kTmemO = kBuffers * 128;
-// Registers: 168 a thread at launch (the most that 384 threads can have); the softmax warps hold a row of 128 scores.
-constexpr int kRegsLaunch = 168, kRegsSoftmax = 208, kRegsOther = 88;
-static_assert(256 * kRegsSoftmax + 128 * kRegsOther <= kThreads * kRegsLaunch, "shares of the launch's registers");
+// Registers: 128 a thread at launch (the most that 512 threads can have); the softmax warps hold a row of 128 scores.
+constexpr int kRegsLaunch = 128, kRegsSoftmax = 200, kRegsOther = 56;
+static_assert(256 * kRegsSoftmax + 256 * kRegsOther <= kThreads * kRegsLaunch, "shares of the launch's registers");
 
 struct PrefillArgs {
     CUtensorMap q_map, k_map, v_map;
@@ -81,16 +83,17 @@ struct Smem {
     static constexpr int kBars = kV + kSlots * kSlab;
     static constexpr int kBarQFull = 0, kBarQEmpty = 2, kBarKFull = 4, kBarKEmpty = kBarKFull + kSlots, kBarVFull = kBarKEmpty + kSlots,
                          kBarVEmpty = kBarVFull + kSlots, kBarS = kBarVEmpty + kSlots, kBarP = kBarS + kBuffers, kBarPv = kBarP + kBuffers,
-                         kBarO = kBarPv + 2, kBarRead = kBarO + 1, kBarTail = kBarRead + 4, kBarRecFull = kBarTail + 1,
+                         kBarO = kBarPv + 2, kBarRead = kBarO + 1, kBarSums = kBarRead + 8, kBarSumsEmpty = kBarSums + 8,
+                         kBarTail = kBarSumsEmpty + 8, kBarRecFull = kBarTail + 1,
                          kBarRecEmpty = kBarRecFull + kRecords, kNumBars = kBarRecEmpty + kRecords;
     static constexpr int kRecs = kBars + kNumBars * 8;
     static constexpr int kRef = kRecs + kRecords * kRecInts * 4;         // the rows' reference
-    static constexpr int kSums = kRef + 128 * 4;                         // {reference, sum} of one warpgroup at an item's end
-    static constexpr int kQueue = kSums + 128 * 8;                       // eight items {blocks, keys} with scores not yet added
+    static constexpr int kSums = kRef + 128 * 4;                         // {reference, sum} of each warpgroup at an item's end, of two items
+    static constexpr int kQueue = kSums + 4 * 128 * 8;                   // eight items {blocks, keys} with scores not yet added
     static constexpr int kTurn = kQueue + 8 * 8;                         // [kRecords][4] whether the warps of a quarter go on
     static constexpr int kMisc = kTurn + kRecords * 4 * 4;               // abort flag, tensor memory address
-    static constexpr int kOut = (kMisc + 16 + 127) & ~127;               // [4][32 rows][32 columns] of output on their way
-    static constexpr int kBytes = kOut + 4 * 2048;
+    static constexpr int kOut = (kMisc + 16 + 127) & ~127;               // [4][32 rows][16 columns] of output on their way
+    static constexpr int kBytes = kOut + 4 * 1024;
 };
 static_assert(Smem<192>::kBytes <= 232448 && Smem<128>::kBytes <= 232448, "shared memory of one CTA");
 
@@ -163,9 +166,9 @@ __device__ __forceinline__ bool find_item(const PrefillArgs &a, Walk &w, long lo
             if (idx < w.base + here) {
                 // head after head, whose items are neighbours (they read the same keys); levels fall, from the highest that the
                 // sequence has in the bucket
-                const long long local = idx - w.base - static_cast<long long>(upto - n) * a.heads;
-                if (local >= 0 && local < static_cast<long long>(n) * a.heads) {         // one lane
-                    const int head = static_cast<int>(local / n), level = min(w.high, s.top) - static_cast<int>(local % n);
+                const int local = static_cast<int>(idx - w.base) - (upto - n) * a.heads;  // (all items are fewer than 2^31)
+                if (local >= 0 && local < n * a.heads) {                                 // one lane
+                    const int head = local / n, level = min(w.high, s.top) - (local - head * n);
                     const int m0 = (s.blocks - 1 - (s.top - level)) << 8;
                     const int rows = min(256, s.nq - m0), off = m0 + s.nk - s.nq;
                     const int see = a.causal ? min(s.nk, max(0, off + rows)) : s.nk;     // keys that the item's last row sees
@@ -431,9 +434,7 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
 }
 
 // Warpgroup `side` takes the tiles g with g % 2 == side of a CTA's sequence; its thread is a row (lane of tensor memory).  The
-// row's reference passes from tile to tile through shared memory; each warpgroup keeps its own part of the sum.  The
-// warpgroup with an item's last tile writes its output, while the other computes the next item's first weights, which it
-// hands over when the output has been read.
+// row's reference passes from tile to tile through shared memory; each warpgroup keeps its own part of the sum.
 template <int DQK, bool FP16>
 __device__ __forceinline__ void softmax_role(const PrefillArgs &a, uint8_t *smem, uint32_t tmem, volatile int *abort_flag, int rank, int warp, int lane) {
     using L = Smem<DQK>;
@@ -442,11 +443,11 @@ __device__ __forceinline__ void softmax_role(const PrefillArgs &a, uint8_t *smem
     const uint32_t t_lane = tmem + (static_cast<uint32_t>(quarter * 32) << 16), o_addr = t_lane + kTmemO;
     float *ref_at = reinterpret_cast<float *>(smem + L::kRef) + lane_row;
     const uint32_t p_bar = map_rank(bars + L::kBarP * 8, 0);  // the even CTA's
-    float2 *sums = reinterpret_cast<float2 *>(smem + L::kSums) + lane_row;
+    float2 *sums = reinterpret_cast<float2 *>(smem + L::kSums) + side * 128 + lane_row;
     const float c = a.scale_log2;
     uint32_t tile = 0, n_items = 0;              // tiles; items with keys
     bool failed = false;
-    // The two warps of a quarter meet at barriers that know no time limit, so they have to take the same items.  Whichever
+    // The two softmax warps of a quarter meet at barriers that know no time limit, so they have to take the same items.  Whichever
     // comes to an item first decides, for both, whether they take it or one of them has given up.
     int *turns = reinterpret_cast<int *>(smem + L::kTurn) + quarter;
     const auto go_on = [&](int it, bool mine) {
@@ -468,8 +469,7 @@ __device__ __forceinline__ void softmax_role(const PrefillArgs &a, uint8_t *smem
             break;
         }
         const volatile int *rec = reinterpret_cast<const int *>(smem + L::kRecs) + slot * kRecInts;
-        const int valid = rec[kRecValid], n = rec[kRecN], nk = rec[kRecNk], off = rec[kRecOff], rows = rec[kRecRows], head = rec[kRecHead],
-                  qrow = rec[kRecQRow];
+        const int valid = rec[kRecValid], n = rec[kRecN], nk = rec[kRecNk], off = rec[kRecOff];
         __syncwarp();
         if (lane == 0) mbar_arrive(bars + (L::kBarRecEmpty + slot) * 8);
         if (!valid) break;
@@ -557,75 +557,105 @@ __device__ __forceinline__ void softmax_role(const PrefillArgs &a, uint8_t *smem
             tmem_st_wait();
             tc_fence_before_sync();
             __syncwarp();
-            // the last item's output has been read before the product that overwrites it can start
-            if (t == 0 && n_items > 0) failed |= !mbar_wait(bars + (L::kBarRead + quarter) * 8, (n_items - 1) & 1, abort_flag);
+            // The last item's output (k - 1) has been read before the product that overwrites it can start.  Two barriers in
+            // turn: what item k - 3 signalled on this one is known to have come.  Either items k - 1 and k - 2 have a tile each, and
+            // this warpgroup waited for k - 3 with the one of k - 2; or they have three, and this tile's scores came behind the
+            // product of a tile of k - 2, which waited for it.
+            if (t == 0 && n_items > 0) {
+                const uint32_t last = n_items - 1;
+                failed |= !mbar_wait(bars + (L::kBarRead + (last & 1) * 4 + quarter) * 8, (last >> 1) & 1, abort_flag);
+            }
             if (lane == 0) mbar_arrive_remote(p_bar + buf * 8);
         }
-        // The item's end.  The sums of both warpgroups go under the later of their references (it only rises).
+        if (n == 0) continue;
         float lx, ly;
         unpack2(l2, lx, ly);
-        const float mine_l = lx + ly;
-        const bool last = n > 0 ? ((tile - 1) & 1) == static_cast<uint32_t>(side) : side == 0;
-        if (!last) {
-            if (n > 0) {
-                *sums = make_float2(m, mine_l);
-                __syncwarp();
-                named_bar_arrive(1 + quarter, 64);
-                ++n_items;
-            }
-            continue;
-        }
-        float2 other = make_float2(-INFINITY, 0.0f);
+        const uint32_t sums_at = (n_items & 1) * 4 + quarter;
+        failed |= !mbar_wait(bars + (L::kBarSumsEmpty + sums_at) * 8, ((n_items >> 1) & 1) ^ 1, abort_flag);
+        sums[(n_items & 1) * 256] = make_float2(m, lx + ly);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bars + (L::kBarSums + sums_at) * 8);
+        ++n_items;
+    }
+    if (tile > 0 && (tile & 1) == static_cast<uint32_t>(side)) named_bar_sync(6 + quarter * 2 - side, 64);      // the last arrival's
+    if (failed && lane == 0) give_up(abort_flag, a.status, kStatusSoftmaxWait);
+}
+
+// The output of an item, while the softmax warps go on with the next one, whose first weights they hand over when this output
+// has been read.  A thread is a row.
+template <int DQK, bool FP16>
+__device__ __forceinline__ void output_role(const PrefillArgs &a, uint8_t *smem, uint32_t tmem, volatile int *abort_flag, int rank, int quarter, int lane) {
+    using L = Smem<DQK>;
+    const uint32_t bars = smem_u32(smem + L::kBars), o_addr = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + kTmemO;
+    const int row = rank * 128 + quarter * 32 + lane;
+    const float2 *sums = reinterpret_cast<const float2 *>(smem + L::kSums) + quarter * 32 + lane;
+    // A warp's rows go through shared memory 16 columns at a time, so that two lanes store 32 consecutive bytes: 16 bytes of
+    // each row at a time, straight from the lanes, take 32 cycles of the load and store unit per instruction.  The loop is not
+    // unrolled: the instruction cache holds the softmax, and a whole row in registers first (88 of them) took 40 % longer
+    // where items are one tile.
+    uint8_t *stage = smem + L::kOut + quarter * 1024;
+    uint4 *put[2] = {reinterpret_cast<uint4 *>(stage + lane * 32 + (lane >> 2 & 1) * 16), reinterpret_cast<uint4 *>(stage + lane * 32 + (~lane >> 2 & 1) * 16)};
+    const uint4 *get = reinterpret_cast<const uint4 *>(stage + (lane >> 1) * 32 + ((lane ^ (lane >> 3)) & 1) * 16);
+    const int first = rank * 128 + quarter * 32 + (lane >> 1);
+    uint32_t n_items = 0;
+    bool ok = true;
+    for (int it = 0;; ++it) {
+        const int slot = it % kRecords;
+        if (!(ok = mbar_wait(bars + (L::kBarRecFull + slot) * 8, (it / kRecords) & 1, abort_flag))) break;
+        const volatile int *rec = reinterpret_cast<const int *>(smem + L::kRecs) + slot * kRecInts;
+        const int valid = rec[kRecValid], n = rec[kRecN], rows = rec[kRecRows], head = rec[kRecHead], qrow = rec[kRecQRow];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bars + (L::kBarRecEmpty + slot) * 8);
+        if (!valid) break;
+        float top = -INFINITY, l = 0.0f;
         if (n > 0) {
-            named_bar_sync(1 + quarter, 64);
-            other = *sums;
+            // the sums of both warpgroups, under the later of their references (it only rises)
+            const uint32_t sums_at = (n_items & 1) * 4 + quarter;
+            if (!(ok = mbar_wait(bars + (L::kBarSums + sums_at) * 8, (n_items >> 1) & 1, abort_flag))) break;
+            const float2 s0 = sums[(n_items & 1) * 256], s1 = sums[(n_items & 1) * 256 + 128];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bars + (L::kBarSumsEmpty + sums_at) * 8);
+            top = fmaxf(s0.x, s1.x);
+            l = top == -INFINITY ? s0.y + s1.y : s0.y * fast_exp2(s0.x - top) + s1.y * fast_exp2(s1.x - top);      // 0, or NaN from NaN
         }
-        const float top = fmaxf(m, other.x);
-        const float l = top == -INFINITY ? mine_l + other.y : mine_l * fast_exp2(m - top) + other.y * fast_exp2(other.x - top);    // 0, or NaN from NaN
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
         if (row < rows && a.lse != nullptr) a.lse[head * a.lse_hs + qrow + row] = l == 0.0f ? -INFINITY : (top + log2f(l)) * kLn2;
         if (n > 0) {
-            failed |= !mbar_wait(bars + L::kBarO * 8, n_items & 1, abort_flag);
+            if (!(ok = mbar_wait(bars + L::kBarO * 8, n_items & 1, abort_flag))) break;
             tc_fence_after_sync();
         }
-        // A warp's rows go through shared memory 32 columns at a time, so that four lanes store 64 consecutive bytes: 16 bytes of
-        // each row at a time, straight from the lanes, take 32 cycles of the load and store unit per instruction.
-        uint8_t *stage = smem + L::kOut + quarter * 2048;
-        const int first = rank * 128 + quarter * 32 + (lane >> 2);
-        uint16_t *dst = static_cast<uint16_t *>(a.out) + (qrow + first) * a.o_ts + head * a.o_hs + (lane & 3) * 8;
-        const bool store = !__any_sync(0xffffffffu, failed);
+        uint16_t *dst = static_cast<uint16_t *>(a.out) + (qrow + first) * a.o_ts + head * a.o_hs + (lane & 1) * 8;
 #pragma unroll 1
-        for (int j = 0; j < 128; j += 32) {
-            uint4 w[4] = {};
+        for (int j = 0; j < 128; j += 16) {
+            uint4 w[2] = {};
             if (n > 0) {
-                uint32_t o[32];
-                tmem_ld_x32_nowait(o_addr + j, o);
-                tmem_ld_wait();
+                uint32_t o[16];
+                tmem_ld_x16(o_addr + j, o);
+                if (j == 112) {
+                    tc_fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bars + (L::kBarRead + (n_items & 1) * 4 + quarter) * 8);
+                }
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
+                for (int e = 0; e < 2; ++e) {
                     uint32_t x[4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i)      // a row without keys: zeros (the accumulator may hold anything)
                         x[i] = l == 0.0f ? 0u : pack16<FP16>(__uint_as_float(o[e * 8 + 2 * i]) * inv, __uint_as_float(o[e * 8 + 2 * i + 1]) * inv);
-                    *reinterpret_cast<uint4 *>(stage + lane * 64 + ((e ^ (lane >> 1)) & 3) * 16) = make_uint4(x[0], x[1], x[2], x[3]);
+                    *put[e] = make_uint4(x[0], x[1], x[2], x[3]);
                 }
                 __syncwarp();
-#pragma unroll
-                for (int e = 0; e < 4; ++e) w[e] = *reinterpret_cast<const uint4 *>(stage + e * 512 + (lane >> 2) * 64 + ((lane ^ (lane >> 3)) & 3) * 16);
-                tc_fence_before_sync();
+                w[0] = get[0];
+                w[1] = get[32];
                 __syncwarp();
-                if (j == 96 && lane == 0) mbar_arrive(bars + (L::kBarRead + quarter) * 8);
             }
-            if (store) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (first + e * 8 < rows) *reinterpret_cast<uint4 *>(dst + e * 8 * a.o_ts + j) = w[e];
-            }
+            for (int e = 0; e < 2; ++e)
+                if (first + e * 16 < rows) *reinterpret_cast<uint4 *>(dst + e * 16 * a.o_ts + j) = w[e];
         }
         if (n > 0) ++n_items;
     }
-    if (tile > 0 && (tile & 1) == static_cast<uint32_t>(side)) named_bar_sync(6 + quarter * 2 - side, 64);      // the last arrival's
-    if (failed && lane == 0) give_up(abort_flag, a.status, kStatusSoftmaxWait);
+    if (!ok && lane == 0) give_up(abort_flag, a.status, kStatusSoftmaxWait);
 }
 
 template <int DQK, bool FP16>
@@ -651,10 +681,12 @@ __global__ void __launch_bounds__(kThreads, 1) dense_prefill_kernel(const __grid
         init(L::kBarP, kBuffers, 8);             // four warps of each CTA
         init(L::kBarPv, 2, 1);
         init(L::kBarO, 1, 1);
-        init(L::kBarRead, 4, 1);
+        init(L::kBarRead, 8, 1);
+        init(L::kBarSums, 8, 2);                 // a warp of each softmax warpgroup
+        init(L::kBarSumsEmpty, 8, 1);
         init(L::kBarTail, 1, 1);
         init(L::kBarRecFull, kRecords, 1);
-        init(L::kBarRecEmpty, kRecords, rank == 0 ? 10 : 9);
+        init(L::kBarRecEmpty, kRecords, rank == 0 ? 14 : 13);
         for (int i = 0; i < kRecords * 4; ++i) reinterpret_cast<int *>(smem + L::kTurn)[i] = 0;
         *abort_flag = 0;
         mbar_init_fence();
@@ -672,6 +704,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_prefill_kernel(const __grid
         if (warp == 8 && rank == 0) mma_role<DQK, FP16>(a, smem, tmem, abort_flag, lane);
         else if (warp == 9) qk_loader_role<DQK>(a, smem, abort_flag, rank, lane);
         else if (warp == 10) v_loader_role<DQK>(a, smem, abort_flag, rank, lane);
+        else if (warp >= 12) output_role<DQK, FP16>(a, smem, tmem, abort_flag, rank, warp & 3, lane);
     }
     tc_fence_before_sync();
     __syncwarp();
