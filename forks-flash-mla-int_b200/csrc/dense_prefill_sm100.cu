@@ -83,7 +83,7 @@ struct Smem {
     static constexpr int kBars = kV + kSlots * kSlab;
     static constexpr int kBarQFull = 0, kBarQEmpty = 2, kBarKFull = 4, kBarKEmpty = kBarKFull + kSlots, kBarVFull = kBarKEmpty + kSlots,
                          kBarVEmpty = kBarVFull + kSlots, kBarS = kBarVEmpty + kSlots, kBarP = kBarS + kBuffers, kBarPv = kBarP + kBuffers,
-                         kBarO = kBarPv + 2, kBarRead = kBarO + 1, kBarSums = kBarRead + 8, kBarSumsEmpty = kBarSums + 8,
+                         kBarO = kBarPv + 4, kBarRead = kBarO + 1, kBarSums = kBarRead + 8, kBarSumsEmpty = kBarSums + 8,
                          kBarTail = kBarSumsEmpty + 8, kBarRecFull = kBarTail + 1,
                          kBarRecEmpty = kBarRecFull + kRecords, kNumBars = kBarRecEmpty + kRecords;
     static constexpr int kRecs = kBars + kNumBars * 8;
@@ -408,7 +408,7 @@ __device__ __forceinline__ void mma_role(const PrefillArgs &a, uint8_t *smem, ui
         if (++o_t == o_n) umma_commit_pair_pred(bars + L::kBarO * 8, go);
         if (find_tile()) score();
         if (!ok) break;
-        umma_commit_pair_pred(bars + (L::kBarPv + ((added - 1) & 1)) * 8, go);
+        umma_commit_pair_pred(bars + (L::kBarPv + ((added - 1) & 3)) * 8, go);
         umma_commit_pair_pred(bars + (L::kBarVEmpty + at) * 8, go);
         if (++at == L::kSlots) {
             at = 0;
@@ -480,6 +480,11 @@ __device__ __forceinline__ void softmax_role(const PrefillArgs &a, uint8_t *smem
         for (int t = 0; t < n; ++t, ++tile) {
             if ((tile & 1) != static_cast<uint32_t>(side)) continue;
             const uint32_t buf = tile % kBuffers, s_addr = t_lane + buf * 128;
+            // The output's barriers take turns over four tiles, and a parity tells only neighbouring phases apart: a wait for the
+            // product of tile - 1 (below) needs to know that the one of tile - 5 has arrived.  So every tile's warp sees the product
+            // of tile - 4 first: it came before these scores in the tensor pipe (no delay), tile's own cannot have come, and the
+            // warp before saw the one of tile - 5 ahead of its arrival at the named barrier.
+            failed |= !mbar_wait(bars + (L::kBarPv + (tile & 3)) * 8, ((tile >> 2) & 1) ^ 1, abort_flag);
             failed |= !mbar_wait(bars + (L::kBarS + buf) * 8, (tile / kBuffers) & 1, abort_flag);
             tc_fence_after_sync();
             uint32_t s[128];
@@ -516,7 +521,7 @@ __device__ __forceinline__ void softmax_role(const PrefillArgs &a, uint8_t *smem
                 // (the warpgroup's first tile of an item, or one of the last two tiles moved a reference)
                 if (t > 0 && __any_sync(0xffffffffu, to != now)) {
                     // everything before this tile has to be in O, nothing behind it can be
-                    failed |= !mbar_wait(bars + (L::kBarPv + ((tile - 1) & 1)) * 8, ((tile - 1) >> 1) & 1, abort_flag);
+                    failed |= !mbar_wait(bars + (L::kBarPv + ((tile - 1) & 3)) * 8, ((tile - 1) >> 2) & 1, abort_flag);
                     tc_fence_after_sync();
                     const float f = to == now ? 1.0f : fast_exp2(now - to);
 #pragma unroll 1
@@ -679,7 +684,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_prefill_kernel(const __grid
         init(L::kBarVEmpty, L::kSlots, 1);
         init(L::kBarS, kBuffers, 1);
         init(L::kBarP, kBuffers, 8);             // four warps of each CTA
-        init(L::kBarPv, 2, 1);
+        init(L::kBarPv, 4, 1);
         init(L::kBarO, 1, 1);
         init(L::kBarRead, 8, 1);
         init(L::kBarSums, 8, 2);                 // a warp of each softmax warpgroup

@@ -266,3 +266,21 @@ def test_many_prompts_of_mixed_lengths(fm):
     kl = [x + rng.choice([0, 0, 1, 200, 700]) for x in ql]
     a = inputs(ql, kl, h=3, seed=18)
     check(fm.dense_mla_prefill(*a), a)
+
+
+@pytest.mark.parametrize("d", [192, 128])
+@pytest.mark.parametrize("q_lens,k_lens", [([700, 1, 390, 1100, 129], None), ([40, 300, 2], [2000, 1500, 1411]), ([30] * 60, [385] * 60)])
+def test_references_that_move_at_every_tile(fm, d, q_lens, k_lens):
+    """Each block of 128 keys scores about 2^9 and more above the one before, in items of one to sixteen blocks, so that the output is
+    moved to a new reference at every tile of every item, and items follow one another on the same pair of CTAs.  The same bits twice."""
+    a = inputs(q_lens, k_lens, h=24, hk=12, d=d, seed=d + len(q_lens), gain=0.25)
+    q, k, _, _, cu_k = a
+    at = torch.arange(k.shape[0], device="cuda") - cu_k[:-1].long().repeat_interleave((cu_k[1:] - cu_k[:-1]).long())
+    # scores climb by 0.05 a key, 6.4 = 9.2 ln 2 a block, in one product (bf16 rounds the largest, 100, by a quarter)
+    q[:, :, 0] = d ** 0.5
+    k[:, :, 0] = (0.05 * at).to(k.dtype)[:, None]
+    one = fm.dense_mla_prefill(*a)
+    check(one, a)
+    for _ in range(20):
+        two = fm.dense_mla_prefill(*a)
+        assert torch.equal(one[0], two[0]) and torch.equal(one[1], two[1])
