@@ -41,6 +41,17 @@ int device_info(DevInfo &out) {
 
 int max_width(const smla_attn_params_t &p) { return p.swa.topk + (p.extra.cache ? p.extra.topk : 0); }
 
+// Whether any element of [batch, wa] at `a`, rows sa apart, is one of [batch, wb] at `b`, rows sb apart; where the two lie between
+// one another with different strides, that counts as well.
+bool share_elements(const float *a, int64_t sa, int64_t wa, const float *b, int64_t sb, int64_t wb, int64_t batch) {
+    if (wa == 0 || wb == 0) return false;
+    const int64_t d = static_cast<int64_t>(reinterpret_cast<uintptr_t>(b) / 4) - static_cast<int64_t>(reinterpret_cast<uintptr_t>(a) / 4);
+    if (d >= (batch - 1) * sa + wa || -d >= (batch - 1) * sb + wb) return false;
+    if (batch == 1 || sa != sb) return true;
+    const int64_t at = ((d % sa) + sa) % sa;     // where b's rows begin in a's
+    return at < wa || at + wb > sa;
+}
+
 }  // namespace
 
 extern "C" {
@@ -229,15 +240,25 @@ int smla_cache_row_weights_workspace(int seqlen_q, int num_heads, size_t *bytes)
 int smla_select_cache_rows(const float *weights, int64_t weights_stride, int width, const int32_t *cache_seqlens,
                            int batch, int budget, int recent, int32_t *rows, int32_t *kept, float *kept_weights,
                            void *stream) {
+    return smla_select_cache_rows_into(weights, weights_stride, width, cache_seqlens, batch, budget, recent, rows, kept, kept_weights,
+                                       budget, budget, stream);
+}
+
+int smla_select_cache_rows_into(const float *weights, int64_t weights_stride, int width, const int32_t *cache_seqlens,
+                                int batch, int budget, int recent, int32_t *rows, int32_t *kept, float *kept_weights,
+                                int64_t kept_weights_stride, int kept_weights_width, void *stream) {
     if (batch < 0 || width < 0 || budget < 1 || recent < 0 || recent > budget || weights_stride < width) return SMLA_EINVAL;
+    if (kept_weights && (kept_weights_width < (width < budget ? width : budget) || kept_weights_stride < kept_weights_width)) return SMLA_EINVAL;
     if (batch == 0) return SMLA_OK;
     if ((width > 0 && !weights) || !cache_seqlens || !rows || !kept) return SMLA_EINVAL;
+    if (kept_weights && share_elements(weights, weights_stride, width, kept_weights, kept_weights_stride, kept_weights_width, batch))
+        return SMLA_EINVAL;
     DevInfo d;
     const int rc = device_info(d);
     if (rc != SMLA_OK) return rc;
     if (d.major != 10) return SMLA_EARCH;
     return smla::launch_select_rows(weights, weights_stride, width, cache_seqlens, batch, budget, recent, rows, kept,
-                                    kept_weights, static_cast<cudaStream_t>(stream));
+                                    kept_weights, kept_weights_stride, kept_weights_width, static_cast<cudaStream_t>(stream));
 }
 
 int smla_compact_cache(const smla_compact_params_t *p, void *stream) {

@@ -39,7 +39,7 @@ __device__ __forceinline__ float key_weight(uint32_t k) { return __uint_as_float
 
 __global__ void __launch_bounds__(kSelThreads, 1) select_rows_kernel(const float *weights, int64_t stride, int width, const int32_t *lens,
                                                                      int budget, int recent, int held, int32_t *rows, int32_t *kept,
-                                                                     float *kept_weights) {
+                                                                     float *kept_weights, int64_t kept_stride, int kept_width) {
     extern __shared__ __align__(16) uint32_t keys[];         // `held` of this CTA's keys, a multiple of 4
     __shared__ unsigned hist[2][256];
     __shared__ unsigned total[256];              // digit d at (255 - d) % 8 * 32 + (255 - d) / 8
@@ -52,13 +52,12 @@ __global__ void __launch_bounds__(kSelThreads, 1) select_rows_kernel(const float
     const int len = min(max(lens[b], 0), width), stay = min(len, budget);
     const float *w = weights + b * stride;
     rows += static_cast<int64_t>(b) * budget;
-    if (kept_weights) kept_weights += static_cast<int64_t>(b) * budget;
+    if (kept_weights) kept_weights += b * kept_stride;
     const int all = rank * kSelThreads + tid, step = ranks * kSelThreads;
     if (all == 0) kept[b] = stay;
-    for (int j = stay + all; j < budget; j += step) {
-        rows[j] = -1;
-        if (kept_weights) kept_weights[j] = 0.0f;
-    }
+    for (int j = stay + all; j < budget; j += step) rows[j] = -1;
+    if (kept_weights)
+        for (int j = stay + all; j < kept_width; j += step) kept_weights[j] = 0.0f;
     const int old = len - recent, want0 = budget - recent;   // of the `old` first rows `want0` stay
     const bool whole = len <= budget;
     if (whole || want0 == 0) {                   // (the whole cluster takes the same way)
@@ -311,7 +310,7 @@ __global__ void __launch_bounds__(kSliceThreads) move_rows_in_place_kernel(const
 }  // namespace
 
 int launch_select_rows(const float *weights, int64_t weights_stride, int width, const int32_t *lens, int batch, int budget,
-                       int recent, int32_t *rows, int32_t *kept, float *kept_weights, cudaStream_t stream) {
+                       int recent, int32_t *rows, int32_t *kept, float *kept_weights, int64_t kept_stride, int kept_width, cudaStream_t stream) {
     // As many CTAs to a sequence as leave each at least 4096 rows and do not ask for more than one per SM (up to 8, the
     // portable cluster size); more than 8 x 48 K rows are partly read from L2 in each pass.
     int ranks = 1;
@@ -334,7 +333,8 @@ int launch_select_rows(const float *weights, int64_t weights_stride, int width, 
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    return static_cast<int>(cudaLaunchKernelEx(&cfg, select_rows_kernel, weights, weights_stride, width, lens, budget, recent, held, rows, kept, kept_weights));
+    return static_cast<int>(cudaLaunchKernelEx(&cfg, select_rows_kernel, weights, weights_stride, width, lens, budget, recent, held, rows, kept, kept_weights,
+                                               kept_stride, kept_width));
 }
 
 int launch_compact(const smla_compact_params_t &p, int, cudaStream_t stream) {

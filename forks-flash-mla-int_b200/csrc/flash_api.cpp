@@ -19,6 +19,7 @@
 #include <torch/csrc/stable/tensor.h>
 #include <torch/headeronly/util/Exception.h>
 
+#include <algorithm>
 #include <cstdint>
 #include <optional>
 #include <string>
@@ -551,8 +552,9 @@ Tensor mla_cache_row_weights(const Tensor &q_in, const Tensor &cache, const Tens
     return weights;
 }
 
-void mla_select_cache_rows(const Tensor &weights_in, const Tensor &lens_in, int64_t budget, int64_t recent, Tensor &rows,
-                           Tensor &kept, Tensor &kept_weights) {
+// `given` fp32 [batch, columns] takes the sums of the rows that stay; without it they are a new tensor [batch, budget].
+void mla_select_cache_rows(const Tensor &weights_in, const Tensor &lens_in, int64_t budget, int64_t recent, const Tensor *given,
+                           Tensor &rows, Tensor &kept, Tensor &kept_weights) {
     const char *what = "MLA cache row selection";
     STD_TORCH_CHECK(weights_in.is_cuda() && weights_in.scalar_type() == ScalarType::Float && weights_in.dim() == 2, what,
                     ": weights must be a float32 CUDA tensor (batch_size, rows)");
@@ -561,16 +563,25 @@ void mla_select_cache_rows(const Tensor &weights_in, const Tensor &lens_in, int6
     check_lens(lens_in, device, B, what);
     STD_TORCH_CHECK(budget >= 1 && budget <= 0x7FFFFFFF && recent >= 0 && recent <= budget, what, ": expected 0 <= recent <= budget and budget >= 1");
     STD_TORCH_CHECK(weights_in.size(1) <= 0x7FFFFFFF && B <= 0x7FFFFFFF, what, ": too many rows");
+    if (given) {
+        const Tensor &w = *given;
+        STD_TORCH_CHECK(on_device(w, device) && w.scalar_type() == ScalarType::Float && w.dim() == 2 && w.size(0) == B &&
+                            (w.size(1) <= 1 || w.stride(1) == 1) && (B <= 1 || w.stride(0) >= w.size(1)) && w.size(1) <= 0x7FFFFFFF &&
+                            w.size(1) >= std::min(weights_in.size(1), budget),
+                        what, ": kept_weights must be a float32 (batch_size, columns) tensor with contiguous rows on the same device, at least "
+                        "min(budget, columns of weights) wide");
+    }
     torch::stable::accelerator::DeviceGuard guard(device);
     const Tensor weights = as_table(weights_in);
     const Tensor lens = lens_in.is_contiguous() ? lens_in : torch::stable::contiguous(lens_in);
     rows = empty_on(device, {B, budget}, aoti_torch_dtype_int32());
     kept = empty_on(device, {B}, aoti_torch_dtype_int32());
-    kept_weights = empty_on(device, {B, budget}, aoti_torch_dtype_float32());
-    check_rc(smla_select_cache_rows(static_cast<const float *>(weights.data_ptr()), row_stride_2d(weights), static_cast<int>(weights.size(1)),
-                                    static_cast<const int32_t *>(lens.data_ptr()), static_cast<int>(B), static_cast<int>(budget),
-                                    static_cast<int>(recent), static_cast<int32_t *>(rows.data_ptr()), static_cast<int32_t *>(kept.data_ptr()),
-                                    static_cast<float *>(kept_weights.data_ptr()), current_stream(device)),
+    kept_weights = given ? *given : empty_on(device, {B, budget}, aoti_torch_dtype_float32());
+    check_rc(smla_select_cache_rows_into(static_cast<const float *>(weights.data_ptr()), row_stride_2d(weights), static_cast<int>(weights.size(1)),
+                                         static_cast<const int32_t *>(lens.data_ptr()), static_cast<int>(B), static_cast<int>(budget),
+                                         static_cast<int>(recent), static_cast<int32_t *>(rows.data_ptr()), static_cast<int32_t *>(kept.data_ptr()),
+                                         static_cast<float *>(kept_weights.data_ptr()), row_stride_2d(kept_weights),
+                                         static_cast<int>(kept_weights.size(1)), current_stream(device)),
              what);
 }
 
@@ -722,10 +733,18 @@ void boxed_add_row_weights(StableIValue *stack, uint64_t, uint64_t) {
 
 void boxed_select_rows(StableIValue *stack, uint64_t, uint64_t) {
     Tensor rows, kept, kept_weights;
-    mla_select_cache_rows(to<Tensor>(stack[0]), to<Tensor>(stack[1]), to<int64_t>(stack[2]), to<int64_t>(stack[3]), rows, kept, kept_weights);
+    mla_select_cache_rows(to<Tensor>(stack[0]), to<Tensor>(stack[1]), to<int64_t>(stack[2]), to<int64_t>(stack[3]), nullptr, rows, kept, kept_weights);
     stack[0] = from(rows);
     stack[1] = from(kept);
     stack[2] = from(kept_weights);
+}
+
+void boxed_select_rows_into(StableIValue *stack, uint64_t, uint64_t) {
+    const Tensor given = to<Tensor>(stack[4]);
+    Tensor rows, kept, kept_weights;
+    mla_select_cache_rows(to<Tensor>(stack[0]), to<Tensor>(stack[1]), to<int64_t>(stack[2]), to<int64_t>(stack[3]), &given, rows, kept, kept_weights);
+    stack[0] = from(rows);
+    stack[1] = from(kept);
 }
 
 void boxed_compact(StableIValue *stack, uint64_t, uint64_t) {
@@ -765,6 +784,7 @@ STABLE_TORCH_LIBRARY(flash_mla, m) {
     m.def("add_mla_cache_row_weights(Tensor q, Tensor kcache, Tensor block_table, Tensor cache_seqlens, Tensor softmax_lse, "
           "float softmax_scale, bool causal, Tensor(a!) weights) -> ()");
     m.def("mla_select_cache_rows(Tensor weights, Tensor cache_seqlens, int budget, int recent) -> (Tensor, Tensor, Tensor)");
+    m.def("mla_select_cache_rows_into(Tensor weights, Tensor cache_seqlens, int budget, int recent, Tensor(a!) kept_weights) -> (Tensor, Tensor)");
     m.def("mla_compact_cache(Tensor(a!) kcache, Tensor block_table, Tensor rows, Tensor kept, Tensor? out_block_table) -> ()");
 }
 
@@ -783,6 +803,7 @@ STABLE_TORCH_LIBRARY_IMPL(flash_mla, CUDA, m) {
     m.impl("mla_cache_row_weights", &boxed_row_weights);
     m.impl("add_mla_cache_row_weights", &boxed_add_row_weights);
     m.impl("mla_select_cache_rows", &boxed_select_rows);
+    m.impl("mla_select_cache_rows_into", &boxed_select_rows_into);
     m.impl("mla_compact_cache", &boxed_compact);
 }
 

@@ -19,7 +19,7 @@ SMLA_ETOOBIG = -5
 EXPORTS = (
     "smla_version", "smla_error_string", "smla_choose_num_splits", "smla_attn_workspace_bytes",
     "smla_decode_plan", "smla_decode_kernel_launches", "smla_decode_kernel_launches_captured", "smla_sparse_mla_decode", "smla_sparse_mla_decode_static_scratch", "smla_sparse_mla_prefill", "smla_dense_mla_decode",
-    "smla_dense_mla_prefill", "smla_cache_row_weights", "smla_cache_row_weights_workspace", "smla_select_cache_rows", "smla_compact_cache",
+    "smla_dense_mla_prefill", "smla_cache_row_weights", "smla_cache_row_weights_workspace", "smla_select_cache_rows", "smla_select_cache_rows_into", "smla_compact_cache",
     "smla_quantize_int8_ds_mla_rows", "smla_write_int8_ds_mla_cache", "smla_write_fp8_ds_mla_cache",
     "smla_read_device_status", "smla_device_status_address",
 )
@@ -204,6 +204,8 @@ def load() -> C.CDLL:
     lib.smla_cache_row_weights_workspace.argtypes = [C.c_int, C.c_int, C.POINTER(C.c_size_t)]
     lib.smla_select_cache_rows.argtypes = [C.c_void_p, C.c_int64, C.c_int, C.c_void_p, C.c_int, C.c_int, C.c_int,
                                            C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]
+    lib.smla_select_cache_rows_into.argtypes = [C.c_void_p, C.c_int64, C.c_int, C.c_void_p, C.c_int, C.c_int, C.c_int,
+                                                C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int, C.c_void_p]
     lib.smla_compact_cache.argtypes = [C.POINTER(SmlaCompactParams), C.c_void_p]
     lib.smla_quantize_int8_ds_mla_rows.argtypes = [C.c_void_p, C.c_int, C.c_int64, C.c_int64, C.c_void_p,
                                                    C.c_void_p, C.c_void_p]

@@ -9,8 +9,16 @@ weights of a window two), none of which synchronises:
 ``mla_compact_cache``       moves those rows to the front of the sequence's pages (or to other pages).
 
 The heads share one latent row, so a row's weight is the sum over all of them.  Rows keep the rotary position they
-were written with.  After the move the sequence has ``kept`` rows; its remaining pages are free, and
-``kept_weights`` are the sums to go on adding to.  No counterpart in the reference.
+were written with.  After the move the sequence has ``kept`` rows; its remaining pages are free.  A program that evicts
+again and again keeps two tensors of sums, each as wide as the table's rows, and lets the selection write one from the
+other, so that the rows appended later have their place in it:
+
+    mla_cache_row_weights(q, k_cache, block_table, cache_seqlens, lse, causal=True, weights=sums)      # every step
+    rows, kept, other = mla_select_cache_rows(sums, cache_seqlens, budget, recent, kept_weights=other)
+    mla_compact_cache(k_cache, block_table, rows, kept)
+    cache_seqlens, sums, other = kept, other, sums
+
+No counterpart in the reference.
 """
 from __future__ import annotations
 
@@ -27,6 +35,7 @@ load_torch_extension()
 _new_weights = torch.ops.flash_mla.mla_cache_row_weights.default
 _add_weights = torch.ops.flash_mla.add_mla_cache_row_weights.default
 _select = torch.ops.flash_mla.mla_select_cache_rows.default
+_select_into = torch.ops.flash_mla.mla_select_cache_rows_into.default
 _compact = torch.ops.flash_mla.mla_compact_cache.default
 
 
@@ -60,8 +69,9 @@ def mla_cache_row_weights(q: torch.Tensor, k_cache: torch.Tensor, block_table: t
         softmax_lse: (batch_size, num_heads_q, seq_len_q) float32 as that call returned it.  A query whose entry is
             -inf saw no row and adds nothing.
         weights: float32 (batch_size, rows) with contiguous rows to add to, in place; the entries behind a
-            sequence's length stay as they are, and rows past the tensor's width are left out.  None: a new
-            tensor with one column per row that ``block_table`` can name, 0 behind each length.
+            sequence's length stay as they are, and rows past the tensor's width are left out (a selection from it
+            would not see them either).  None: a new tensor with one column per row that ``block_table`` can name, 0
+            behind each length.
 
     Returns ``weights``.  The sums are formed in a fixed order: the same call gives the same bits."""
     try:
@@ -93,26 +103,41 @@ def _check_weights_call(q, k_cache, block_table, cache_seqlens, softmax_lse, wei
         raise ValueError(f"expected weights float32 [{batch}, rows], got {weights.dtype} {tuple(weights.shape)}")
 
 
-def mla_select_cache_rows(weights: torch.Tensor, cache_seqlens: torch.Tensor, budget: int,
-                          recent: int = 0) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+def mla_select_cache_rows(weights: torch.Tensor, cache_seqlens: torch.Tensor, budget: int, recent: int = 0,
+                          kept_weights: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """The rows of each sequence that stay when at most ``budget`` of them may.
 
     A sequence of at most ``budget`` rows (its length counts up to the width of ``weights``) keeps them all.  A
     longer one keeps its last ``recent`` rows and, of those in front of them, the ``budget - recent`` with the
     largest weights; the lower row goes first where weights are equal, and a NaN counts as less than every number.
 
-    Arguments: weights float32 (batch_size, rows); cache_seqlens int32 (batch_size,); 0 <= recent <= budget.
+    Rows past the width of ``weights`` are not seen, and they would be the newest: it has to be as wide as the longest
+    sequence, in a second eviction too.
+
+    Arguments: weights float32 (batch_size, rows); cache_seqlens int32 (batch_size,); 0 <= recent <= budget;
+        kept_weights: float32 (batch_size, columns) with contiguous rows to write the weights of the rows that stay to, 0
+            behind them: sums to go on adding to, as wide as the table's rows so that rows appended later have their
+            place.  At least min(budget, rows) columns; it must not overlap ``weights``.  None: a new tensor with budget columns.
 
     Returns rows int32 (batch_size, budget), ascending, -1 behind the last; kept int32 (batch_size,), how many;
-    kept_weights float32 (batch_size, budget), their weights, 0 behind."""
+    kept_weights, their weights, 0 behind."""
     try:
-        return _select(weights, cache_seqlens, budget, recent)
+        if kept_weights is None:
+            return _select(weights, cache_seqlens, budget, recent)
+        rows, kept = _select_into(weights, cache_seqlens, budget, recent, kept_weights)
+        return rows, kept, kept_weights
     except (RuntimeError, NotImplementedError):
         if weights.dim() != 2 or weights.dtype != torch.float32:
             raise ValueError(f"expected weights float32 [batch, rows], got {weights.dtype} {tuple(weights.shape)}")
         _check_lens("cache_seqlens", cache_seqlens, weights.shape[0])
         if budget < 1 or not 0 <= recent <= budget:
             raise ValueError(f"expected 0 <= recent <= budget and budget >= 1, got budget {budget}, recent {recent}")
+        if kept_weights is not None:
+            batch, columns = weights.shape[0], min(budget, weights.shape[1])
+            if kept_weights.dim() != 2 or kept_weights.shape[0] != batch or kept_weights.dtype != torch.float32 or kept_weights.shape[1] < columns:
+                raise ValueError(f"expected kept_weights float32 [{batch}, at least {columns}], got {kept_weights.dtype} {tuple(kept_weights.shape)}")
+            if kept_weights.untyped_storage().data_ptr() == weights.untyped_storage().data_ptr():
+                raise ValueError("kept_weights must not overlap weights")
         raise
 
 

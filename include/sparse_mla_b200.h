@@ -268,10 +268,18 @@ SMLA_API int smla_cache_row_weights(const smla_row_weights_params_t *params, voi
  *    length (clamped to `width`) is at most the budget; else the last `recent` rows and, of the rows in front of
  *    them, the budget - recent with the largest weights, the lower row first where weights are equal (-0 equals
  *    0, a NaN counts as less than every number).  rows[b, :kept[b]] ascend, -1 behind; kept_weights (may be NULL)
- *    are their weights, 0 behind.  0 <= recent <= budget, budget >= 1. */
+ *    are their weights, 0 behind.  0 <= recent <= budget, budget >= 1.
+ *    Rows past `width` are not seen: `weights` has to be as wide as the longest sequence, or its newest rows go.  So
+ *    sums that are to be added to, and selected from again, after rows were appended need room for those rows: the second
+ *    form writes them as rows of kept_weights_width columns (at least min(width, budget)), kept_weights_stride elements apart, 0
+ *    behind the kept ones.  kept_weights must not overlap weights (SMLA_EINVAL). */
 SMLA_API int smla_select_cache_rows(const float *weights, int64_t weights_stride, int width,
                                     const int32_t *cache_seqlens, int batch, int budget, int recent, int32_t *rows,
                                     int32_t *kept, float *kept_weights, void *stream);
+SMLA_API int smla_select_cache_rows_into(const float *weights, int64_t weights_stride, int width,
+                                         const int32_t *cache_seqlens, int batch, int budget, int recent, int32_t *rows,
+                                         int32_t *kept, float *kept_weights, int64_t kept_weights_stride,
+                                         int kept_weights_width, void *stream);
 
 /* 3. smla_compact_cache: row rows[b, j] of sequence b (through block_table) becomes its row j (through
  *    out_block_table), j < kept[b].  rows [batch, budget] contiguous.  With out_block_table == block_table and

@@ -49,11 +49,12 @@ def cache_row_weights(q, k_cache, block_table, cache_seqlens, lse, scale=None, c
     return w, bound
 
 
-def select_cache_rows(weights, cache_seqlens, budget, recent=0):
+def select_cache_rows(weights, cache_seqlens, budget, recent=0, columns=None):
+    """-> rows, kept, kept weights in ``columns`` (default: budget) columns."""
     b, width = weights.shape
     rows = torch.full((b, budget), -1, dtype=torch.int32)
     kept = torch.zeros(b, dtype=torch.int32)
-    vals = torch.zeros(b, budget, dtype=torch.float32)
+    vals = torch.zeros(b, budget if columns is None else columns, dtype=torch.float32)
     for i in range(b):
         n = min(max(int(cache_seqlens[i]), 0), width)
         w = weights[i].cpu().tolist()

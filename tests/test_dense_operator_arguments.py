@@ -267,3 +267,39 @@ def test_compact_oracle():
     assert torch.equal(got[2, 0], cache[2, 1]) and torch.equal(got[2, 1], cache[0, 0])
     assert torch.equal(got[3, 0], cache[3, 1]) and (got[3, 1] == 0).all()       # page 9 does not exist
     assert torch.equal(got[0], cache[0]) and torch.equal(got[1], cache[1])
+
+
+# ----------------------------------------------------------------------------- sums with room for rows appended later
+def test_select_refuses_places_for_the_kept_weights(fm):
+    w, lens = torch.zeros(2, 9), torch.zeros(2, dtype=torch.int32)
+    for bad in (torch.zeros(2, 3), torch.zeros(1, 9), torch.zeros(2, 9, dtype=torch.float64), torch.zeros(18), w, w[:, :5]):
+        with pytest.raises(ValueError):
+            fm.mla_select_cache_rows(w, lens, 4, 1, kept_weights=bad)
+
+
+@pytest.mark.parametrize("change,code", [
+    (dict(kept_width=3), SMLA_EINVAL), (dict(kept_stride=7), SMLA_EINVAL), (dict(width=2, stride=2, kept_width=1), SMLA_EINVAL),
+    (dict(vals=FAKE), SMLA_EINVAL), (dict(vals=FAKE + 4 * 40), SMLA_EINVAL), (dict(vals=FAKE - 4 * 40), SMLA_EINVAL),
+    (dict(vals=FAKE + 4 * 7, stride=16, kept_stride=16), SMLA_EINVAL), (dict(vals=FAKE + 4 * 9, stride=16, kept_stride=16), SMLA_EINVAL),
+    (dict(vals=FAKE - 4 * 7, stride=16, kept_stride=16), SMLA_EINVAL), (dict(vals=FAKE + 4 * 8, stride=16, kept_stride=15), SMLA_EINVAL),
+    (dict(batch=0), SMLA_OK), (dict(budget=0), SMLA_EINVAL),
+])
+def test_select_into_c_refusals(abi, change, code):
+    """weights [8, 8], kept_weights [8, 8] that are too narrow, the same, or partly the same."""
+    a = dict(weights=FAKE, stride=8, width=8, lens=FAKE, batch=8, budget=4, recent=0, rows=FAKE, kept=FAKE, vals=FAKE + 4096, kept_stride=8,
+             kept_width=8)
+    a.update(change)
+    assert abi.load().smla_select_cache_rows_into(a["weights"], a["stride"], a["width"], a["lens"], a["batch"], a["budget"], a["recent"],
+                                                  a["rows"], a["kept"], a["vals"], a["kept_stride"], a["kept_width"], None) == code
+
+
+def test_two_evictions_of_the_oracle_keep_the_newest_rows():
+    """200 rows, 64 stay; 40 more; the second choice is among 104 and has the last 16, where the sums have room for them."""
+    g = torch.Generator().manual_seed(2)
+    sums = torch.rand(1, 320, generator=g)
+    sums[:, 200:] = 0
+    rows, kept, sums = oracle.select_cache_rows(sums, torch.tensor([200]), 64, 16, columns=320)
+    assert sums.shape == (1, 320) and (sums[:, 64:] == 0).all()
+    sums[:, :104] += torch.rand(1, 104, generator=g)
+    rows, kept, sums = oracle.select_cache_rows(sums, torch.tensor([104]), 64, 16, columns=320)
+    assert rows[0, -16:].tolist() == list(range(88, 104)) and kept.tolist() == [64]

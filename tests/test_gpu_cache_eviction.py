@@ -589,3 +589,110 @@ def test_the_first_call_of_a_process_may_be_a_captured_one(fm):
     root = os.path.dirname(os.path.dirname(os.path.abspath(fm.__file__)))
     run = subprocess.run([sys.executable, "-c", _FIRST_CALL], env={**os.environ, "PYTHONPATH": root}, capture_output=True, text=True, timeout=300)
     assert run.returncode == 0 and "captured" in run.stdout, run.stderr[-2000:]
+
+
+# ----------------------------------------------------------------------------- sums that go on through several evictions
+@pytest.mark.parametrize("lens,width,budget,recent,columns", [([90, 300, 0, 5, 64], 300, 64, 16, 300), ([700, 699, 1], 700, 333, 333, 1000),
+                                                              ([50, 9], 60, 500, 4, 60), ([9000, 8192], 9000, 700, 1, 20001), ([40], 40, 40, 0, 41)])
+def test_select_into_sums_with_room_to_grow(fm, lens, width, budget, recent, columns):
+    g = torch.Generator(device="cuda").manual_seed(width)
+    w = torch.rand(len(lens), width, generator=g, device="cuda")
+    w[w < 0.3] = 0
+    lens = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    buf = torch.full((len(lens), columns + 7), float("nan"), device="cuda")
+    place = buf[:, 3:3 + columns]
+    rows, kept, sums = fm.mla_select_cache_rows(w, lens, budget, recent, kept_weights=place)
+    want = oracle.select_cache_rows(w, lens, budget, recent, columns=columns)
+    assert sums.data_ptr() == place.data_ptr()
+    assert torch.equal(rows.cpu(), want[0]) and torch.equal(kept.cpu(), want[1]) and torch.equal(place.cpu(), want[2])
+    assert torch.isnan(buf[:, :3]).all() and torch.isnan(buf[:, 3 + columns:]).all()
+
+
+def test_select_into_the_other_half_of_a_buffer(fm):
+    """Rows of the two that lie between one another do not overlap; the sums themselves, or a part of them, are refused."""
+    buf = torch.rand(5, 2, 100, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda")
+    w = buf[:, 0].clone()
+    lens = torch.tensor([100, 70, 30, 0, 99], dtype=torch.int32, device="cuda")
+    want = oracle.select_cache_rows(w, lens, 40, 5, columns=100)
+    fm.mla_select_cache_rows(buf[:, 0], lens, 40, 5, kept_weights=buf[:, 1])
+    assert torch.equal(buf[:, 1].cpu(), want[2]) and torch.equal(buf[:, 0], w)
+    for bad in (buf[:, 0], buf[:, 0, 50:], buf.view(5, 200)[:, 40:150]):
+        with pytest.raises(ValueError):
+            fm.mla_select_cache_rows(buf[:, 0], lens, 40, 5, kept_weights=bad)
+    assert torch.equal(buf[:, 0], w)
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_several_evictions_with_rows_appended_between(fm, captured):
+    """What the guide's loop does: rows are appended, a decode step, its weights added to the sums, and an eviction, four times.
+    Each row has a number; the host follows which numbers a sequence has and what weights each has had."""
+    h, page, per, budget, recent, fresh, rounds = 4, 16, 20, 64, 16, 40, 4
+    g = torch.Generator(device="cuda").manual_seed(7)
+    lens = [200, 30, 130]
+    b = len(lens)
+    table = torch.randperm(b * per, generator=torch.Generator().manual_seed(8)).to(torch.int32).view(b, per).cuda()
+    cache = torch.zeros(b * per, page, 1, 576, dtype=torch.bfloat16, device="cuda")
+    rows_of = torch.randn(b, 200 + fresh * rounds, 576, generator=g, device="cuda").to(torch.bfloat16)     # by number
+    seqlens = torch.tensor(lens, dtype=torch.int32, device="cuda")
+
+    def put(i, first, numbers):
+        r = torch.arange(first, first + len(numbers), device="cuda")
+        cache[table[i].long()[r // page], r % page, 0] = rows_of[i, numbers]
+    numbers = [list(range(n)) for n in lens]
+    for i in range(b):
+        put(i, 0, numbers[i])
+    sums = [torch.zeros(b, per * page, device="cuda"), torch.full((b, per * page), float("nan"), device="cuda")]
+    had = [dict.fromkeys(x, 0.0) for x in numbers]
+    q = torch.randn(b, 1, h, 576, generator=g, device="cuda").to(torch.bfloat16)
+    meta, splits = fm.get_mla_metadata(seqlens, h, 1)
+
+    def step(now, other):
+        _, lse = fm.flash_mla_with_kvcache(q, cache, table, seqlens, 512, meta, splits, causal=True)
+        fm.mla_cache_row_weights(q, cache, table, seqlens, lse, causal=True, weights=now)
+        rows, kept, _ = fm.mla_select_cache_rows(now, seqlens, budget, recent, kept_weights=other)
+        fm.mla_compact_cache(cache, table, rows, kept)
+        return lse, rows, kept
+    graphs = []
+    if captured:
+        keep = cache.clone()
+        step(sums[0], sums[1])
+        sums[0].zero_()
+        cache.copy_(keep)
+        torch.cuda.synchronize()
+        for k in range(2):
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                graphs.append((graph, step(sums[k], sums[1 - k])))
+    for turn in range(rounds):
+        now, other = sums[turn & 1], sums[1 - (turn & 1)]
+        q.copy_(torch.randn(q.shape, generator=g, device="cuda"))
+        if turn:
+            for i in range(b):
+                new = list(range(200 + fresh * turn, 200 + fresh * (turn + 1)))
+                put(i, len(numbers[i]), new)
+                numbers[i] += new
+                had[i].update(dict.fromkeys(new, 0.0))
+            seqlens.copy_(torch.tensor([len(x) for x in numbers], dtype=torch.int32))
+        if captured:
+            graphs[turn & 1][0].replay()
+            lse, rows, kept = graphs[turn & 1][1]
+        else:
+            lse, rows, kept = step(now, other)
+        torch.cuda.synchronize()
+        assert kept.tolist() == [min(len(x), budget) for x in numbers]
+        for i in range(b):
+            s = rows_of[i, numbers[i]].double() @ q[i, 0].double().t() * 576 ** -0.5
+            for number, x in zip(numbers[i], torch.exp(s - lse[i, :, 0].double()).sum(1).tolist()):
+                had[i][number] += x
+            total = torch.tensor([had[i][x] for x in numbers[i]], dtype=torch.float64)
+            # d 2^-23 scale sum |q k| and the like, as in check_weights: far below 1e-3 of a weight, four times
+            assert ((now[i, : total.numel()].cpu().double() - total).abs() <= 1e-3 * total + 1e-9).all()
+            ids, _, vals = oracle.select_cache_rows(now[i:i + 1], seqlens[i:i + 1], budget, recent, columns=per * page)
+            m = int(kept[i])
+            assert rows[i, :m].tolist() == ids[0, :m].tolist() and torch.equal(other[i].cpu(), vals[0])
+            before = len(numbers[i])
+            assert rows[i, :m].tolist()[-min(recent, m):] == list(range(before - min(recent, m), before))      # the newest are there
+            numbers[i] = [numbers[i][r] for r in rows[i, :m].tolist()]
+            r = torch.arange(m, device="cuda")
+            assert torch.equal(cache[table[i].long()[r // page], r % page, 0], rows_of[i, numbers[i]])
+        seqlens.copy_(kept)
