@@ -55,21 +55,22 @@ __global__ void __launch_bounds__(kSelThreads, 1) select_rows_kernel(const float
     if (kept_weights) kept_weights += b * kept_stride;
     const int all = rank * kSelThreads + tid, step = ranks * kSelThreads;
     if (all == 0) kept[b] = stay;
-    for (int j = stay + all; j < budget; j += step) rows[j] = -1;
+    // (a budget, a width or a length may be up to 2^31 - 1, so what is counted up to them in steps is 64 bits wide)
+    for (int64_t j = static_cast<int64_t>(stay) + all; j < budget; j += step) rows[j] = -1;
     if (kept_weights)
-        for (int j = stay + all; j < kept_width; j += step) kept_weights[j] = 0.0f;
+        for (int64_t j = static_cast<int64_t>(stay) + all; j < kept_width; j += step) kept_weights[j] = 0.0f;
     const int old = len - recent, want0 = budget - recent;   // of the `old` first rows `want0` stay
     const bool whole = len <= budget;
     if (whole || want0 == 0) {                   // (the whole cluster takes the same way)
         const int first = whole ? 0 : old;
-        for (int j = all; j < stay; j += step) {
-            rows[j] = first + j;
+        for (int64_t j = all; j < stay; j += step) {
+            rows[j] = static_cast<int>(first + j);
             if (kept_weights) kept_weights[j] = w[first + j];
         }
         return;
     }
     // this CTA's part: whole multiples of 32 rows, in rank order
-    const int part = ((old + ranks - 1) / ranks + 31) & ~31;
+    const int part = ((old - 1) / ranks + 32) & ~31;
     const int lo = min(rank * part, old), n = min(part, old - lo);
     const float *mine = w + lo;
     const auto key_at = [&](int j) { return j < held ? keys[j] : weight_key(__ldg(mine + j)); };
@@ -221,8 +222,8 @@ __global__ void __launch_bounds__(kSelThreads, 1) select_rows_kernel(const float
             above += __popc(up[e]);
         }
     }
-    for (int j = all; j < recent; j += step) {
-        rows[want0 + j] = old + j;
+    for (int64_t j = all; j < recent; j += step) {
+        rows[want0 + j] = static_cast<int>(old + j);
         if (kept_weights) kept_weights[want0 + j] = w[old + j];
     }
     if (ranks > 1) cluster.sync();               // no CTA may end while another reads its sums
@@ -316,7 +317,7 @@ int launch_select_rows(const float *weights, int64_t weights_stride, int width, 
     int ranks = 1;
     while (ranks < 8 && width / (ranks * 2) >= 4096 && static_cast<int64_t>(batch) * ranks * 2 <= 148) ranks *= 2;
     while (ranks < 8 && width / ranks > kMaxKeys) ranks *= 2;
-    const int part = ((width + ranks - 1) / ranks + 31) & ~31, held = std::min(part, kMaxKeys);
+    const int part = (std::max(width - 1, 0) / ranks + 32) & ~31, held = std::min(part, kMaxKeys);
     if (static_cast<int64_t>(batch) * ranks > 0x7FFFFFFFLL) return SMLA_ETOOBIG;
     static KernelSetup setup;
     int *status;                                 // (this kernel waits for nothing that could fail to come)

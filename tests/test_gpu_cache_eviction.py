@@ -696,3 +696,36 @@ def test_several_evictions_with_rows_appended_between(fm, captured):
             r = torch.arange(m, device="cuda")
             assert torch.equal(cache[table[i].long()[r // page], r % page, 0], rows_of[i, numbers[i]])
         seqlens.copy_(kept)
+
+
+_MOST = 2 ** 31 - 1
+
+
+@pytest.mark.parametrize("width,budget,recent", [(100, _MOST, 0), (_MOST, _MOST, 3), (_MOST, 5000, 77), (_MOST, _MOST - 1, _MOST - 2)])
+def test_select_sizes_up_to_the_largest_integer(fm, width, budget, recent):
+    """"Keep all" said as the largest budget; the longest row of weights; the most recent rows.  Up to 27 GB."""
+    w = torch.zeros(1, width, device="cuda")
+    heavy = torch.arange(3, width - 1, max(1, width // 40), device="cuda")[:37]
+    w[0, heavy] = torch.rand(heavy.numel(), device="cuda") + 1.0
+    lens = torch.tensor([width], dtype=torch.int32, device="cuda")
+    rows, kept, sums = fm.mla_select_cache_rows(w, lens, budget, recent)
+    stay, old = min(width, budget), width - recent
+    assert int(kept) == stay and rows.shape == sums.shape == (1, budget)
+    if width <= budget:
+        front = torch.arange(min(stay, 10 ** 6), device="cuda")
+    else:                                                     # heavy ones first, then the lowest of the zeros
+        top = heavy[heavy < old]
+        lowest = torch.arange(min(old, budget), device="cuda")
+        lowest = lowest[~torch.isin(lowest, top)]
+        pick = torch.cat([top[torch.sort(w[0, top], descending=True, stable=True).indices], lowest])[: budget - recent]
+        front = pick.sort().values
+        assert rows[0, budget - recent] == old and rows[0, -1] == width - 1
+        step = rows[0, budget - recent:]
+        for at in range(0, recent, 1 << 28):
+            piece = step[at:at + (1 << 28)]
+            assert torch.equal(piece, torch.arange(old + at, old + at + piece.numel(), dtype=torch.int32, device="cuda"))
+    assert torch.equal(rows[0, : front.numel()].long(), front) and torch.equal(sums[0, : front.numel()], w[0, front])
+    if width == budget:
+        assert torch.equal(sums, w) and int(rows[0, -1]) == width - 1
+    for at in range(stay, budget, 1 << 28):
+        assert (rows[0, at:at + (1 << 28)] == -1).all() and (sums[0, at:at + (1 << 28)] == 0).all()
