@@ -214,6 +214,7 @@ int smla_cache_row_weights(const smla_row_weights_params_t *p, void *stream) {
         !p->k_cache || p->num_blocks == 0 || (p->max_blocks_per_seq > 0 && !p->block_table))
         return SMLA_EINVAL;
     if (static_cast<int64_t>(p->num_blocks) * p->page_block_size > 0x7FFFFFFFLL ||
+        p->weights_width > 0x7FFFFFFF - 1024 ||  // the kernel counts in ints to the end of a tile of rows or a piece of columns
         static_cast<int64_t>(p->seqlen_q) * p->num_heads > 0x7FFFFFFFLL / 1024 ||
         static_cast<int64_t>(p->batch) * p->seqlen_q * p->num_heads > 0x7FFFFFFFLL - 256)
         return SMLA_ETOOBIG;

@@ -252,7 +252,7 @@ typedef struct smla_row_weights_params {
     const int32_t *cache_seqlens;         /* [batch]                                                             */
     float *weights;                       /* fp32 [batch, weights_width]                                         */
     int64_t weights_stride;               /* elements between sequences                                          */
-    int32_t weights_width;                /* rows past it are left out                                           */
+    int32_t weights_width;                /* rows past it are left out; at most 2^31 - 1025 (else SMLA_ETOOBIG)  */
     int32_t accumulate;
     void *workspace;                      /* 16-byte aligned scratch of smla_cache_row_weights_workspace bytes, which lets
                                              windows of more than 128 (position, head) pairs use every SM; NULL or less:

@@ -303,3 +303,15 @@ def test_two_evictions_of_the_oracle_keep_the_newest_rows():
     sums[:, :104] += torch.rand(1, 104, generator=g)
     rows, kept, sums = oracle.select_cache_rows(sums, torch.tensor([104]), 64, 16, columns=320)
     assert rows[0, -16:].tolist() == list(range(88, 104)) and kept.tolist() == [64]
+
+
+@pytest.mark.parametrize("width,code", [(2 ** 31 - 1, SMLA_ETOOBIG), (2 ** 31 - 1024, SMLA_ETOOBIG)])
+def test_row_weights_refuse_rows_that_a_tile_would_count_past_an_int(abi, width, code):
+    """A tile of 256 rows and a piece of 1024 columns that begin in front of 2^31 must end there."""
+    p = abi.SmlaRowWeightsParams()
+    vals = dict(batch=1, seqlen_q=1, num_heads=4, head_dim=576, softmax_scale=0.1, q=FAKE, softmax_lse=FAKE, k_cache=FAKE,
+                k_block_stride=16 * 1152, k_row_stride=1152, num_blocks=5, page_block_size=16, max_blocks_per_seq=2, block_table=FAKE,
+                block_table_stride=2, cache_seqlens=FAKE, weights=FAKE, weights_stride=width, weights_width=width)
+    for k, v in vals.items():
+        setattr(p, k, v)
+    assert abi.load().smla_cache_row_weights(ctypes.byref(p), None) == code
