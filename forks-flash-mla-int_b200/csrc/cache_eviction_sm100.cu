@@ -238,11 +238,17 @@ __device__ __forceinline__ const uint8_t *row_at(const smla_compact_params_t &p,
     return static_cast<const uint8_t *>(p.cache) + page * p.block_stride + (row - col * p.page_block_size) * p.row_stride;
 }
 
+// Rows of sequence b that have a place to go to.
+__device__ __forceinline__ int rows_to_move(const smla_compact_params_t &p, int b) {
+    const int64_t places = static_cast<int64_t>(p.out_max_blocks_per_seq) * p.page_block_size;
+    return static_cast<int>(min(static_cast<int64_t>(min(max(__ldg(p.kept + b), 0), p.budget)), places));
+}
+
 // To other pages: a warp takes four rows, works out their addresses once and has all their pieces in flight together (three
 // of 16 bytes a lane and row: 1152 bytes are 2.25).  Bound by HBM, 2 x row_bytes a row.
 constexpr int kMoveWarps = 8, kMoveRows = 4, kMoveTurn = 3;
 __global__ void __launch_bounds__(kMoveWarps * 32) move_rows_kernel(const smla_compact_params_t p) {
-    const int b = blockIdx.y, n = min(max(__ldg(p.kept + b), 0), p.budget), lane = threadIdx.x & 31;
+    const int b = blockIdx.y, n = rows_to_move(p, b), lane = threadIdx.x & 31;
     const int j0 = (blockIdx.x * kMoveWarps + (threadIdx.x >> 5)) * kMoveRows;
     if (j0 >= n) return;
     const uint8_t *src = nullptr;
@@ -281,14 +287,14 @@ __global__ void __launch_bounds__(kMoveWarps * 32) move_rows_kernel(const smla_c
 // so what a later turn reads has not been written yet.  Bound by the latency of a turn, a load and a barrier.
 constexpr int kSlice = 64, kSliceThreads = 512, kTurnRows = 512, kTurnPieces = kTurnRows / (kSliceThreads / (kSlice / 16));
 __global__ void __launch_bounds__(kSliceThreads) move_rows_in_place_kernel(const smla_compact_params_t p) {
-    const int b = blockIdx.y, n = min(max(p.kept[b], 0), p.budget);
+    const int b = blockIdx.y, n = rows_to_move(p, b);
     const int at = blockIdx.x * kSlice + (threadIdx.x % (kSlice / 16)) * 16;
     const int32_t *rows = p.rows + static_cast<int64_t>(b) * p.budget, *table = p.block_table + b * p.block_table_stride;
-    for (int j0 = 0; j0 < n; j0 += kTurnRows) {
+    for (int64_t j0 = 0; j0 < n; j0 += kTurnRows) {            // (n may be near 2^31)
         uint4 x[kTurnPieces];
 #pragma unroll
         for (int e = 0; e < kTurnPieces; ++e) {
-            const int j = j0 + e * (kTurnRows / kTurnPieces) + threadIdx.x / (kSlice / 16);
+            const int64_t j = j0 + e * (kTurnRows / kTurnPieces) + threadIdx.x / (kSlice / 16);
             x[e] = make_uint4(0, 0, 0, 0);
             if (j < n && at < p.row_bytes) {
                 const uint8_t *src = row_at(p, table, p.max_blocks_per_seq, __ldg(rows + j));
@@ -298,9 +304,9 @@ __global__ void __launch_bounds__(kSliceThreads) move_rows_in_place_kernel(const
         __syncthreads();
 #pragma unroll
         for (int e = 0; e < kTurnPieces; ++e) {
-            const int j = j0 + e * (kTurnRows / kTurnPieces) + threadIdx.x / (kSlice / 16);
+            const int64_t j = j0 + e * (kTurnRows / kTurnPieces) + threadIdx.x / (kSlice / 16);
             if (j < n && at < p.row_bytes) {
-                uint8_t *dst = const_cast<uint8_t *>(row_at(p, table, p.out_max_blocks_per_seq, j));
+                uint8_t *dst = const_cast<uint8_t *>(row_at(p, table, p.out_max_blocks_per_seq, static_cast<int>(j)));
                 if (dst) *reinterpret_cast<uint4 *>(dst + at) = x[e];
             }
         }

@@ -729,3 +729,16 @@ def test_select_sizes_up_to_the_largest_integer(fm, width, budget, recent):
         assert torch.equal(sums, w) and int(rows[0, -1]) == width - 1
     for at in range(stay, budget, 1 << 28):
         assert (rows[0, at:at + (1 << 28)] == -1).all() and (sums[0, at:at + (1 << 28)] == 0).all()
+
+
+@pytest.mark.parametrize("in_place", [True, False])
+def test_compact_with_the_largest_budget(fm, in_place):
+    """The rows of a selection that was told to keep all, and a count that says so too: what the table has places for is moved."""
+    kw, spare = paged([75], h=1, d=64, page=16, seed=61, extra=5)
+    out = None if in_place else spare.view(1, 5).cuda()
+    rows = torch.full((1, _MOST), -1, dtype=torch.int32, device="cuda")
+    rows[0, :60] = torch.arange(15, 75, device="cuda")
+    kept = torch.tensor([_MOST], dtype=torch.int32, device="cuda")
+    want = oracle.compact_cache(kw["k_cache"], kw["block_table"], rows[:, :96].cpu(), torch.tensor([96]), out)
+    fm.mla_compact_cache(kw["k_cache"], kw["block_table"], rows, kept, out_block_table=out)
+    assert same_bytes(kw["k_cache"], want)
