@@ -244,57 +244,21 @@ __device__ __forceinline__ int rows_to_move(const smla_compact_params_t &p, int 
     return static_cast<int>(min(static_cast<int64_t>(min(max(__ldg(p.kept + b), 0), p.budget)), places));
 }
 
-// To other pages: a warp takes four rows, works out their addresses once and has all their pieces in flight together (three
-// of 16 bytes a lane and row: 1152 bytes are 2.25).  Bound by HBM, 2 x row_bytes a row.
-constexpr int kMoveWarps = 8, kMoveRows = 4, kMoveTurn = 3;
-__global__ void __launch_bounds__(kMoveWarps * 32) move_rows_kernel(const smla_compact_params_t p) {
-    const int b = blockIdx.y, n = rows_to_move(p, b), lane = threadIdx.x & 31;
-    const int j0 = (blockIdx.x * kMoveWarps + (threadIdx.x >> 5)) * kMoveRows;
-    if (j0 >= n) return;
-    const uint8_t *src = nullptr;
-    uint8_t *dst = nullptr;
-    if (lane < kMoveRows && j0 + lane < n) {
-        const int row = __ldg(p.rows + static_cast<int64_t>(b) * p.budget + j0 + lane);
-        src = row_at(p, p.block_table + b * p.block_table_stride, p.max_blocks_per_seq, row);
-        dst = const_cast<uint8_t *>(row_at(p, p.out_block_table + b * p.out_block_table_stride, p.out_max_blocks_per_seq, j0 + lane));
-    }
-    const uint8_t *from[kMoveRows];
-    uint8_t *to[kMoveRows];
-#pragma unroll
-    for (int r = 0; r < kMoveRows; ++r) {
-        from[r] = reinterpret_cast<const uint8_t *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src), r));
-        to[r] = reinterpret_cast<uint8_t *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), r));
-    }
-    for (int at = lane * 16; at < p.row_bytes; at += kMoveTurn * 512) {
-        uint4 x[kMoveRows][kMoveTurn];
-#pragma unroll
-        for (int r = 0; r < kMoveRows; ++r)
-#pragma unroll
-            for (int e = 0; e < kMoveTurn; ++e) {
-                x[r][e] = make_uint4(0, 0, 0, 0);
-                if (from[r] && at + e * 512 < p.row_bytes) x[r][e] = __ldcs(reinterpret_cast<const uint4 *>(from[r] + at + e * 512));
-            }
-#pragma unroll
-        for (int r = 0; r < kMoveRows; ++r)
-#pragma unroll
-            for (int e = 0; e < kMoveTurn; ++e)
-                if (to[r] && at + e * 512 < p.row_bytes) *reinterpret_cast<uint4 *>(to[r] + at + e * 512) = x[r][e];
-    }
-}
-
 // Inside their own pages: a CTA takes 64 bytes of all rows of a sequence (slices of a row do not touch one another) and
 // moves 512 rows at a time, all their loads in front of all their stores.  A row's source index is at least its target's,
 // so what a later turn reads has not been written yet.  Bound by the latency of a turn, a load and a barrier.
-constexpr int kSlice = 64, kSliceThreads = 512, kTurnRows = 512, kTurnPieces = kTurnRows / (kSliceThreads / (kSlice / 16));
-__global__ void __launch_bounds__(kSliceThreads) move_rows_in_place_kernel(const smla_compact_params_t p) {
-    const int b = blockIdx.y, n = rows_to_move(p, b);
-    const int at = blockIdx.x * kSlice + (threadIdx.x % (kSlice / 16)) * 16;
-    const int32_t *rows = p.rows + static_cast<int64_t>(b) * p.budget, *table = p.block_table + b * p.block_table_stride;
+constexpr int kSlice = 64, kTurnRows = 512;
+template <int THREADS>
+__device__ __forceinline__ void move_slice_in_place(const smla_compact_params_t &p, int b, int n, int slice) {
+    constexpr int kStep = THREADS / (kSlice / 16), kPieces = kTurnRows / kStep;
+    const int at = slice * kSlice + (threadIdx.x % (kSlice / 16)) * 16;
+    const int32_t *rows = p.rows + static_cast<int64_t>(b) * p.budget, *table = p.block_table + b * p.block_table_stride,
+                  *out_table = p.out_block_table + b * p.out_block_table_stride;
     for (int64_t j0 = 0; j0 < n; j0 += kTurnRows) {            // (n may be near 2^31)
-        uint4 x[kTurnPieces];
+        uint4 x[kPieces];
 #pragma unroll
-        for (int e = 0; e < kTurnPieces; ++e) {
-            const int64_t j = j0 + e * (kTurnRows / kTurnPieces) + threadIdx.x / (kSlice / 16);
+        for (int e = 0; e < kPieces; ++e) {
+            const int64_t j = j0 + e * kStep + threadIdx.x / (kSlice / 16);
             x[e] = make_uint4(0, 0, 0, 0);
             if (j < n && at < p.row_bytes) {
                 const uint8_t *src = row_at(p, table, p.max_blocks_per_seq, __ldg(rows + j));
@@ -303,14 +267,80 @@ __global__ void __launch_bounds__(kSliceThreads) move_rows_in_place_kernel(const
         }
         __syncthreads();
 #pragma unroll
-        for (int e = 0; e < kTurnPieces; ++e) {
-            const int64_t j = j0 + e * (kTurnRows / kTurnPieces) + threadIdx.x / (kSlice / 16);
+        for (int e = 0; e < kPieces; ++e) {
+            const int64_t j = j0 + e * kStep + threadIdx.x / (kSlice / 16);
             if (j < n && at < p.row_bytes) {
-                uint8_t *dst = const_cast<uint8_t *>(row_at(p, table, p.out_max_blocks_per_seq, static_cast<int>(j)));
+                uint8_t *dst = const_cast<uint8_t *>(row_at(p, out_table, p.out_max_blocks_per_seq, static_cast<int>(j)));
                 if (dst) *reinterpret_cast<uint4 *>(dst + at) = x[e];
             }
         }
         __syncthreads();                         // the next turn's loads come behind these stores of the whole CTA
+    }
+}
+
+constexpr int kSliceThreads = 512;
+__global__ void __launch_bounds__(kSliceThreads) move_rows_in_place_kernel(const smla_compact_params_t p) {
+    const int b = blockIdx.y;
+    move_slice_in_place<kSliceThreads>(p, b, rows_to_move(p, b), blockIdx.x);
+}
+
+// To other pages: a warp takes four rows, works out their addresses once and has all their pieces in flight together (three
+// of 16 bytes a lane and row: 1152 bytes are 2.25).  Bound by HBM, 2 x row_bytes a row.
+// A sequence whose target table names some of the source's pages in their own place (a copy of the table, or a table that
+// goes on with new pages) moves in place there: its rows are taken in order, by the first CTAs.
+constexpr int kMoveWarps = 8, kMoveRows = 4, kMoveTurn = 3;
+__global__ void __launch_bounds__(kMoveWarps * 32) move_rows_kernel(const smla_compact_params_t p) {
+    const int b = blockIdx.y, lane = threadIdx.x & 31, slices = (p.row_bytes + kSlice - 1) / kSlice;
+    const int32_t *table = p.block_table + b * p.block_table_stride, *out_table = p.out_block_table + b * p.out_block_table_stride;
+    // the first pages are compared while the count of rows is on its way
+    const int places = min(min(p.max_blocks_per_seq, p.out_max_blocks_per_seq), (p.budget - 1) / p.page_block_size + 1);
+    const auto same_page = [&](int c) {
+        const int page = __ldg(out_table + c);
+        return page == __ldg(table + c) && page >= 0 && page < p.num_blocks;
+    };
+    bool own = static_cast<int>(threadIdx.x) < places && same_page(threadIdx.x);
+    const int n = rows_to_move(p, b), j0 = (blockIdx.x * kMoveWarps + (threadIdx.x >> 5)) * kMoveRows;
+    if (n == 0 || (blockIdx.x >= slices && blockIdx.x * static_cast<int64_t>(kMoveWarps * kMoveRows) >= n)) return;
+    const uint8_t *src = nullptr;
+    uint8_t *dst = nullptr;
+    if (lane < kMoveRows && j0 < n && j0 + lane < n) {
+        const int row = __ldg(p.rows + static_cast<int64_t>(b) * p.budget + j0 + lane);
+        src = row_at(p, table, p.max_blocks_per_seq, row);
+        dst = const_cast<uint8_t *>(row_at(p, out_table, p.out_max_blocks_per_seq, j0 + lane));
+    }
+    const int columns = min(places, (n - 1) / p.page_block_size + 1);
+    own &= static_cast<int>(threadIdx.x) < columns;
+    for (int c = threadIdx.x + kMoveWarps * 32; c < columns; c += kMoveWarps * 32) own |= same_page(c);
+    const uint8_t *from[kMoveRows];
+    uint8_t *to[kMoveRows];
+#pragma unroll
+    for (int r = 0; r < kMoveRows; ++r) {
+        from[r] = reinterpret_cast<const uint8_t *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src), r));
+        to[r] = reinterpret_cast<uint8_t *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), r));
+    }
+    uint4 x[kMoveRows][kMoveTurn];
+    const auto load = [&](int at) {
+#pragma unroll
+        for (int r = 0; r < kMoveRows; ++r)
+#pragma unroll
+            for (int e = 0; e < kMoveTurn; ++e) {
+                x[r][e] = make_uint4(0, 0, 0, 0);
+                if (from[r] && at + e * 512 < p.row_bytes) x[r][e] = __ldcs(reinterpret_cast<const uint4 *>(from[r] + at + e * 512));
+            }
+    };
+    load(lane * 16);                             // in flight while the CTA learns whether they may be stored
+    if (__syncthreads_or(own)) {
+        if (blockIdx.x < slices) move_slice_in_place<kMoveWarps * 32>(p, b, n, blockIdx.x);
+        return;
+    }
+    for (int at = lane * 16; at < p.row_bytes;) {
+#pragma unroll
+        for (int r = 0; r < kMoveRows; ++r)
+#pragma unroll
+            for (int e = 0; e < kMoveTurn; ++e)
+                if (to[r] && at + e * 512 < p.row_bytes) *reinterpret_cast<uint4 *>(to[r] + at + e * 512) = x[r][e];
+        at += kMoveTurn * 512;
+        if (at < p.row_bytes) load(at);
     }
 }
 
@@ -350,8 +380,8 @@ int launch_compact(const smla_compact_params_t &p, int, cudaStream_t stream) {
         move_rows_in_place_kernel<<<dim3(static_cast<unsigned>((p.row_bytes + kSlice - 1) / kSlice), static_cast<unsigned>(p.batch)), kSliceThreads, 0, stream>>>(p);
     } else {
         constexpr int per_block = kMoveWarps * kMoveRows;
-        move_rows_kernel<<<dim3(static_cast<unsigned>((static_cast<int64_t>(p.budget) + per_block - 1) / per_block), static_cast<unsigned>(p.batch)),
-                           kMoveWarps * 32, 0, stream>>>(p);
+        const int64_t blocks = std::max<int64_t>((static_cast<int64_t>(p.budget) + per_block - 1) / per_block, (p.row_bytes + kSlice - 1) / kSlice);
+        move_rows_kernel<<<dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(p.batch)), kMoveWarps * 32, 0, stream>>>(p);
     }
     return static_cast<int>(cudaGetLastError());
 }

@@ -145,9 +145,10 @@ def mla_compact_cache(k_cache: torch.Tensor, block_table: torch.Tensor, rows: to
                       out_block_table: Optional[torch.Tensor] = None) -> None:
     """Move row ``rows[b, j]`` of sequence b to its row j, for j < kept[b], inside ``k_cache``.
 
-    ``block_table`` names the pages that the rows are in, ``out_block_table`` the pages that they go to.  None, or
-    ``block_table`` itself or its first columns, moves them to the front of their own pages, which needs ascending
-    ``rows`` (as ``mla_select_cache_rows`` returns them); other pages must not be among those read.  No page may be
+    ``block_table`` names the pages that the rows are in, ``out_block_table`` the pages that they go to.  None moves
+    them to the front of their own pages, and so does a table that names a sequence's pages in the columns in which
+    ``block_table`` has them (``block_table`` itself, its first columns, a copy); this needs ascending ``rows`` (as
+    ``mla_select_cache_rows`` returns them).  All other target pages must not be among those read.  No page may be
     written for two sequences: a page that sequences share (a common prefix) has to be left to the others by moving to new pages.
     Rows of the cache that are not written keep their contents.
 

@@ -282,9 +282,9 @@ SMLA_API int smla_select_cache_rows_into(const float *weights, int64_t weights_s
                                          int kept_weights_width, void *stream);
 
 /* 3. smla_compact_cache: row rows[b, j] of sequence b (through block_table) becomes its row j (through
- *    out_block_table), j < kept[b].  rows [batch, budget] contiguous.  With out_block_table == block_table and
- *    the same stride the rows move inside their own pages: rows must then ascend, with rows[b, j] >= j (as
- *    selected above).  Otherwise the
+ *    out_block_table), j < kept[b].  rows [batch, budget] contiguous.  Where out_block_table names a page in the same
+ *    column as block_table (the same table, a copy of it, or one that goes on with other pages), the rows of that sequence
+ *    move inside their own pages: they must then ascend, with rows[b, j] >= j (as selected above).  All other
  *    pages written must not be among the pages read.  In both cases no page may be written for two sequences (or
  *    twice for one).  A source row outside the table or the cache is a zero row; a target outside is left out.
  *    row_bytes, strides and base are multiples of 16. */

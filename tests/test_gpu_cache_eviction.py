@@ -742,3 +742,41 @@ def test_compact_with_the_largest_budget(fm, in_place):
     want = oracle.compact_cache(kw["k_cache"], kw["block_table"], rows[:, :96].cpu(), torch.tensor([96]), out)
     fm.mla_compact_cache(kw["k_cache"], kw["block_table"], rows, kept, out_block_table=out)
     assert same_bytes(kw["k_cache"], want)
+
+
+def _same_pages(table, spare, per, kind):
+    """Targets that name the source's pages in their own columns: all of them, the first or the last half, those of some sequences."""
+    out = spare.view(table.shape[0], per).clone() if kind != "all" else table[:, :per].cpu().clone()
+    own = table[:, :per].cpu()
+    if kind == "first":
+        out[:, : per // 2] = own[:, : per // 2]
+    elif kind == "last":
+        out[:, per // 2:] = own[:, per // 2:]
+    elif kind == "some":
+        out[::2] = own[::2]
+    return out.cuda()
+
+
+@pytest.mark.parametrize("kind", ["all", "first", "last", "some"])
+@pytest.mark.parametrize("page,d,lens,budget", [(16, 64, [20000, 9000, 11000], 8000), (1, 40, [3000, 2000, 2500], 1111), (100, 8, [700, 2000, 1000], 600),
+                                                (64, 576, [9000, 5000, 7001], 4096)])
+def test_compact_to_a_copy_of_the_own_pages(fm, kind, page, d, lens, budget):
+    per = (budget + page - 1) // page
+    kw, spare = paged(lens, h=1, d=d, page=page, seed=page, extra=per * len(lens))
+    rows, kept = ascending(lens, budget, page)
+    out = _same_pages(kw["block_table"], spare, per, kind)
+    want = oracle.compact_cache(kw["k_cache"], kw["block_table"], rows, kept, out)
+    start = kw["k_cache"].clone()
+    for _ in range(5):
+        kw["k_cache"].copy_(start)
+        fm.mla_compact_cache(kw["k_cache"], kw["block_table"], rows, kept, out_block_table=out)
+        assert same_bytes(kw["k_cache"], want)
+
+
+def test_compact_to_a_copy_of_a_table_with_other_strides(fm):
+    lens, budget = [5000, 3000], 2000
+    kw, _ = paged(lens, h=1, d=64, page=16, seed=71)
+    rows, kept = ascending(lens, budget, 72)
+    want = oracle.compact_cache(kw["k_cache"], kw["block_table"], rows, kept)
+    fm.mla_compact_cache(kw["k_cache"], kw["block_table"], rows, kept, out_block_table=kw["block_table"].t().contiguous().t())
+    assert same_bytes(kw["k_cache"], want)
