@@ -238,6 +238,13 @@ __device__ __forceinline__ const uint8_t *row_at(const smla_compact_params_t &p,
     return static_cast<const uint8_t *>(p.cache) + page * p.block_stride + (row - col * p.page_block_size) * p.row_stride;
 }
 
+// This block's sequence; the grid's last two dimensions count them.
+__device__ __forceinline__ int sequence_of_block() { return static_cast<int>(blockIdx.z * gridDim.y + blockIdx.y); }
+dim3 sequence_grid(int64_t blocks, int batch) {
+    constexpr int most = 65535;
+    return dim3(static_cast<unsigned>(blocks), std::min(batch, most), (batch - 1) / most + 1);
+}
+
 // Rows of sequence b that have a place to go to.
 __device__ __forceinline__ int rows_to_move(const smla_compact_params_t &p, int b) {
     const int64_t places = static_cast<int64_t>(p.out_max_blocks_per_seq) * p.page_block_size;
@@ -280,8 +287,8 @@ __device__ __forceinline__ void move_slice_in_place(const smla_compact_params_t 
 
 constexpr int kSliceThreads = 512;
 __global__ void __launch_bounds__(kSliceThreads) move_rows_in_place_kernel(const smla_compact_params_t p) {
-    const int b = blockIdx.y;
-    move_slice_in_place<kSliceThreads>(p, b, rows_to_move(p, b), blockIdx.x);
+    const int b = sequence_of_block();
+    if (b < p.batch) move_slice_in_place<kSliceThreads>(p, b, rows_to_move(p, b), blockIdx.x);
 }
 
 // To other pages: a warp takes four rows, works out their addresses once and has all their pieces in flight together (three
@@ -290,7 +297,8 @@ __global__ void __launch_bounds__(kSliceThreads) move_rows_in_place_kernel(const
 // goes on with new pages) moves in place there: its rows are taken in order, by the first CTAs.
 constexpr int kMoveWarps = 8, kMoveRows = 4, kMoveTurn = 3;
 __global__ void __launch_bounds__(kMoveWarps * 32) move_rows_kernel(const smla_compact_params_t p) {
-    const int b = blockIdx.y, lane = threadIdx.x & 31, slices = (p.row_bytes + kSlice - 1) / kSlice;
+    const int b = sequence_of_block(), lane = threadIdx.x & 31, slices = (p.row_bytes + kSlice - 1) / kSlice;
+    if (b >= p.batch) return;
     const int32_t *table = p.block_table + b * p.block_table_stride, *out_table = p.out_block_table + b * p.out_block_table_stride;
     // the first pages are compared while the count of rows is on its way
     const int places = min(min(p.max_blocks_per_seq, p.out_max_blocks_per_seq), (p.budget - 1) / p.page_block_size + 1);
@@ -375,13 +383,12 @@ int launch_select_rows(const float *weights, int64_t weights_stride, int width, 
 }
 
 int launch_compact(const smla_compact_params_t &p, int, cudaStream_t stream) {
-    if (p.batch > 65535) return SMLA_ETOOBIG;
     if (p.out_block_table == p.block_table && (p.batch <= 1 || p.out_block_table_stride == p.block_table_stride)) {
-        move_rows_in_place_kernel<<<dim3(static_cast<unsigned>((p.row_bytes + kSlice - 1) / kSlice), static_cast<unsigned>(p.batch)), kSliceThreads, 0, stream>>>(p);
+        move_rows_in_place_kernel<<<sequence_grid((p.row_bytes + kSlice - 1) / kSlice, p.batch), kSliceThreads, 0, stream>>>(p);
     } else {
         constexpr int per_block = kMoveWarps * kMoveRows;
         const int64_t blocks = std::max<int64_t>((static_cast<int64_t>(p.budget) + per_block - 1) / per_block, (p.row_bytes + kSlice - 1) / kSlice);
-        move_rows_kernel<<<dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(p.batch)), kMoveWarps * 32, 0, stream>>>(p);
+        move_rows_kernel<<<sequence_grid(blocks, p.batch), kMoveWarps * 32, 0, stream>>>(p);
     }
     return static_cast<int>(cudaGetLastError());
 }

@@ -780,3 +780,20 @@ def test_compact_to_a_copy_of_a_table_with_other_strides(fm):
     want = oracle.compact_cache(kw["k_cache"], kw["block_table"], rows, kept)
     fm.mla_compact_cache(kw["k_cache"], kw["block_table"], rows, kept, out_block_table=kw["block_table"].t().contiguous().t())
     assert same_bytes(kw["k_cache"], want)
+
+
+@pytest.mark.parametrize("in_place", [True, False])
+def test_compact_more_sequences_than_a_grid_counts_in_one_dimension(fm, in_place):
+    n, page = 140001, 8
+    g = torch.Generator(device="cuda").manual_seed(81)
+    cache = torch.randn(2 * n, page, 1, 8, generator=g, device="cuda").to(torch.bfloat16)
+    table = torch.randperm(2 * n, generator=g, device="cuda").to(torch.int32)
+    table, out = table[:n, None], None if in_place else table[n:, None]
+    rows = torch.tensor([1, 4, 5], dtype=torch.int32, device="cuda").repeat(n, 1)
+    kept = torch.randint(0, 4, (n,), generator=g, device="cuda").to(torch.int32)
+    want = cache.clone()
+    for j in range(3):
+        live = kept > j
+        want[(table if in_place else out)[live, 0].long(), j] = cache[table[live, 0].long(), (1, 4, 5)[j]]
+    fm.mla_compact_cache(cache, table, rows, kept, out_block_table=out)
+    assert same_bytes(cache, want)
