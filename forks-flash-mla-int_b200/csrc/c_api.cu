@@ -259,7 +259,7 @@ int smla_select_cache_rows_into(const float *weights, int64_t weights_stride, in
     if (rc != SMLA_OK) return rc;
     if (d.major != 10) return SMLA_EARCH;
     return smla::launch_select_rows(weights, weights_stride, width, cache_seqlens, batch, budget, recent, rows, kept,
-                                    kept_weights, kept_weights_stride, kept_weights_width, static_cast<cudaStream_t>(stream));
+                                    kept_weights, kept_weights_stride, kept_weights_width, d.sm_count, static_cast<cudaStream_t>(stream));
 }
 
 int smla_compact_cache(const smla_compact_params_t *p, void *stream) {
@@ -278,7 +278,7 @@ int smla_compact_cache(const smla_compact_params_t *p, void *stream) {
     const int rc = device_info(d);
     if (rc != SMLA_OK) return rc;
     if (d.major != 10) return SMLA_EARCH;
-    return smla::launch_compact(*p, d.sm_count, static_cast<cudaStream_t>(stream));
+    return smla::launch_compact(*p, static_cast<cudaStream_t>(stream));
 }
 
 int smla_sparse_mla_prefill(const smla_attn_params_t *p, void *stream) {

@@ -355,11 +355,12 @@ __global__ void __launch_bounds__(kMoveWarps * 32) move_rows_kernel(const smla_c
 }  // namespace
 
 int launch_select_rows(const float *weights, int64_t weights_stride, int width, const int32_t *lens, int batch, int budget,
-                       int recent, int32_t *rows, int32_t *kept, float *kept_weights, int64_t kept_stride, int kept_width, cudaStream_t stream) {
+                       int recent, int32_t *rows, int32_t *kept, float *kept_weights, int64_t kept_stride, int kept_width, int sm_count,
+                       cudaStream_t stream) {
     // As many CTAs to a sequence as leave each at least 4096 rows and do not ask for more than one per SM (up to 8, the
     // portable cluster size); more than 8 x 48 K rows are partly read from L2 in each pass.
     int ranks = 1;
-    while (ranks < 8 && width / (ranks * 2) >= 4096 && static_cast<int64_t>(batch) * ranks * 2 <= 148) ranks *= 2;
+    while (ranks < 8 && width / (ranks * 2) >= 4096 && static_cast<int64_t>(batch) * ranks * 2 <= sm_count) ranks *= 2;
     while (ranks < 8 && width / ranks > kMaxKeys) ranks *= 2;
     const int part = (std::max(width - 1, 0) / ranks + 32) & ~31, held = std::min(part, kMaxKeys);
     if (static_cast<int64_t>(batch) * ranks > 0x7FFFFFFFLL) return SMLA_ETOOBIG;
@@ -382,7 +383,7 @@ int launch_select_rows(const float *weights, int64_t weights_stride, int width, 
                                                kept_stride, kept_width));
 }
 
-int launch_compact(const smla_compact_params_t &p, int, cudaStream_t stream) {
+int launch_compact(const smla_compact_params_t &p, cudaStream_t stream) {
     if (p.out_block_table == p.block_table && (p.batch <= 1 || p.out_block_table_stride == p.block_table_stride)) {
         move_rows_in_place_kernel<<<sequence_grid((p.row_bytes + kSlice - 1) / kSlice, p.batch), kSliceThreads, 0, stream>>>(p);
     } else {

@@ -38,8 +38,9 @@ int launch_dense_prefill(const smla_prefill_params_t &p, int sm_count, cudaStrea
 int launch_row_weights(const smla_row_weights_params_t &p, int sm_count, cudaStream_t stream);
 size_t row_weights_workspace(int seqlen_q, int num_heads, int sm_count);
 int launch_select_rows(const float *weights, int64_t weights_stride, int width, const int32_t *lens, int batch, int budget,
-                       int recent, int32_t *rows, int32_t *kept, float *kept_weights, int64_t kept_stride, int kept_width, cudaStream_t stream);
-int launch_compact(const smla_compact_params_t &p, int sm_count, cudaStream_t stream);
+                       int recent, int32_t *rows, int32_t *kept, float *kept_weights, int64_t kept_stride, int kept_width, int sm_count,
+                       cudaStream_t stream);
+int launch_compact(const smla_compact_params_t &p, cudaStream_t stream);
 
 int read_and_clear_device_status(int *status_out);
 int device_status_address(int **addr_out);
