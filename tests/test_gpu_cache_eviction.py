@@ -797,3 +797,29 @@ def test_compact_more_sequences_than_a_grid_counts_in_one_dimension(fm, in_place
         want[(table if in_place else out)[live, 0].long(), j] = cache[table[live, 0].long(), (1, 4, 5)[j]]
     fm.mla_compact_cache(cache, table, rows, kept, out_block_table=out)
     assert same_bytes(cache, want)
+
+
+# ----------------------------------------------------------------------------- the columns beside the sums
+@pytest.mark.parametrize("s_q,h", [(1, 16), (2, 40), (5, 60), (33, 20)])
+@pytest.mark.parametrize("width", [1, 150, 256, 513, 1100, 5000])
+def test_weights_touch_nothing_beside_them(fm, s_q, h, width):
+    """Added to, and written with zeros behind the rows, inside a wider buffer: its other columns keep their bits."""
+    from flash_mla import c_abi
+    lib = c_abi.load()
+    kw, _ = paged([700, 0, 130, 1], s_q=s_q, h=h, seed=width)
+    lse = lse_of(kw, True)
+    buf = torch.rand(4, width + 13, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda")
+    before, w = buf.clone(), buf[:, 5:5 + width]
+    got = fm.mla_cache_row_weights(**kw, softmax_lse=lse, causal=True, weights=w)
+    assert torch.equal(buf[:, :5], before[:, :5]) and torch.equal(buf[:, 5 + width:], before[:, 5 + width:])
+    check_weights(got, kw, lse, True, weights=before[:, 5:5 + width])
+    need = ctypes.c_size_t(0)
+    assert lib.smla_cache_row_weights_workspace(s_q, h, ctypes.byref(need)) == 0
+    scratch = torch.empty(need.value + 16, dtype=torch.uint8, device="cuda")
+    for given in ((None, 0), (scratch.data_ptr(), need.value)):
+        buf.copy_(before)
+        assert lib.smla_cache_row_weights(ctypes.byref(_weights_params(c_abi, kw, lse, w, *given)), torch.cuda.current_stream().cuda_stream) == 0
+        assert torch.equal(buf[:, :5], before[:, :5]) and torch.equal(buf[:, 5 + width:], before[:, 5 + width:])
+        check_weights(w, kw, lse, True)
+        for b, n in enumerate((700, 0, 130, 1)):
+            assert (w[b, n:] == 0).all()
