@@ -433,6 +433,12 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
     return r;
 }
 
+// Weights are 2^kLift times exp(s - m).  A weight may be 2^8 before the reference moves, and fp16 holds 2^15: what is above
+// that is given to the small ones, which fp16 drops below 2^-25.  A key far below the row's largest adds next to nothing,
+// but 10^5 of them at 2^-26 are 0.2 % of the output, and the sum counts them.  bf16 has the exponents of fp32.
+template <bool FP16>
+constexpr float kLift = FP16 ? 7.0f : 0.0f;
+
 // Warpgroup `side` takes the tiles g with g % 2 == side of a CTA's sequence; its thread is a row (lane of tensor memory).  The
 // row's reference passes from tile to tile through shared memory; each warpgroup keeps its own part of the sum.
 template <int DQK, bool FP16>
@@ -540,7 +546,7 @@ __device__ __forceinline__ void softmax_role(const PrefillArgs &a, uint8_t *smem
                 __syncwarp();
             }
             named_bar_arrive(5 + quarter * 2 + side, 64);    // the warp with the next tile's rows waits there
-            const float ref = m == -INFINITY ? 0.0f : -m;
+            const float ref = m == -INFINITY ? 0.0f : kLift<FP16> - m;
             const uint64_t c2 = pack2(c, c), ref2 = pack2(ref, ref);
             uint64_t la = l2, lb = 0;
 #pragma unroll
@@ -624,7 +630,7 @@ __device__ __forceinline__ void output_role(const PrefillArgs &a, uint8_t *smem,
             l = top == -INFINITY ? s0.y + s1.y : s0.y * fast_exp2(s0.x - top) + s1.y * fast_exp2(s1.x - top);      // 0, or NaN from NaN
         }
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        if (row < rows && a.lse != nullptr) a.lse[head * a.lse_hs + qrow + row] = l == 0.0f ? -INFINITY : (top + log2f(l)) * kLn2;
+        if (row < rows && a.lse != nullptr) a.lse[head * a.lse_hs + qrow + row] = l == 0.0f ? -INFINITY : (top - kLift<FP16> + log2f(l)) * kLn2;
         if (n > 0) {
             if (!(ok = mbar_wait(bars + L::kBarO * 8, n_items & 1, abort_flag))) break;
             tc_fence_after_sync();

@@ -13,6 +13,7 @@ Tolerances, from the arithmetic (u = eps / 2 of the type: 2^-8 bf16, 2^-11 fp16)
 The lse is off by the weights' factor, n 2^-23 and the rounding of its own size, 2^-22 |lse|.
 """
 import ctypes
+import math
 
 import pytest
 import torch
@@ -284,3 +285,24 @@ def test_references_that_move_at_every_tile(fm, d, q_lens, k_lens):
     for _ in range(20):
         two = fm.dense_mla_prefill(*a)
         assert torch.equal(one[0], two[0]) and torch.equal(one[1], two[1])
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("below", [17.0, 18.5, 20.0])
+def test_many_keys_far_below_the_largest(fm, dt, below):
+    """One key outweighs the 300000 others, which together are up to 1 % of the row, each of them near or below the smallest fp16 number.  With
+    v = 0 for the one and 1 for the others the output is their share.  Off it, relative: the roundings of a weight and of the output, u
+    each (all weights are alike, so nothing averages out); an fp16 weight of 2^7 e^-below is subnormal, 2^-25 at most, so 2^-32
+    e^below; the sum of the weights has eight partial sums of n / 8 terms, each rounded to 2^-24 of the sum, the product
+    n / 16 steps cut off at 2^-23: n 2^-26 together; the exponent, 32 x 2^-23, and the exponential less than 2^-17."""
+    n, d = 300000, 128
+    q = torch.zeros(1, 1, d, dtype=dt, device="cuda")
+    k = torch.zeros(n, 1, d, dtype=dt, device="cuda")
+    v = torch.ones(n, 1, 128, dtype=dt, device="cuda")
+    q[..., 0], k[12345, 0, 0], v[12345] = 1.0, below, 0.0
+    out, lse = fm.dense_mla_prefill(q, k, v, cu([1]), cu([n]), softmax_scale=1.0, causal=False)
+    rest = (n - 1) * math.exp(-below)
+    share = rest / (1 + rest)
+    tol = 2 * torch.finfo(dt).eps / 2 + n * 2.0 ** -26 + 2.0 ** -17 + (2.0 ** -32 * math.exp(below) if dt == torch.float16 else 0.0)
+    assert (out.double() - share).abs().max() <= tol * share, f"{float(out.double().mean()):.4e} for {share:.4e}"
+    assert (lse.double() - (below + math.log1p(rest))).abs().max() <= n * 2.0 ** -27 + 2.0 ** -17
