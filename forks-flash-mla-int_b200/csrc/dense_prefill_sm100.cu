@@ -236,6 +236,10 @@ __device__ __forceinline__ void qk_loader_role(const PrefillArgs &a, uint8_t *sm
             __syncwarp();
         }
     }
+    // What the products still signal to this CTA has to have come before it may end.
+    for (uint32_t i = block > static_cast<uint32_t>(L::kSlots) ? block - L::kSlots : 0; ok && i < block; ++i)
+        ok = mbar_wait(bars + (L::kBarKEmpty + i % L::kSlots) * 8, (i / L::kSlots) & 1, abort_flag);
+    for (uint32_t i = nq > 2 ? nq - 2 : 0; ok && i < nq; ++i) ok = mbar_wait(bars + (L::kBarQEmpty + (i & 1)) * 8, (i >> 1) & 1, abort_flag);
     if (!ok) {
         // Another role gave up, or this one.  The copies in flight have to land before the CTA may end; the odd CTA's are
         // counted by the even one, for which it waits at the end.
@@ -294,6 +298,8 @@ __device__ __forceinline__ void v_loader_role(const PrefillArgs &a, uint8_t *sme
             }
         }
     }
+    for (uint32_t i = block > static_cast<uint32_t>(L::kSlots) ? block - L::kSlots : 0; ok && i < block; ++i)      // as the other loader
+        ok = mbar_wait(bars + (L::kBarVEmpty + i % L::kSlots) * 8, (i / L::kSlots) & 1, abort_flag);
     if (!ok) {
         if (lane == 0) give_up(abort_flag, a.status, kStatusGatherWait);
         __syncwarp();
@@ -588,7 +594,11 @@ __device__ __forceinline__ void softmax_role(const PrefillArgs &a, uint8_t *smem
         if (lane == 0) mbar_arrive(bars + (L::kBarSums + sums_at) * 8);
         ++n_items;
     }
-    if (tile > 0 && (tile & 1) == static_cast<uint32_t>(side)) named_bar_sync(6 + quarter * 2 - side, 64);      // the last arrival's
+    if (tile > 0 && (tile & 1) == static_cast<uint32_t>(side)) {
+        named_bar_sync(6 + quarter * 2 - side, 64);          // the last arrival's
+        for (uint32_t i = tile > 4 ? tile - 4 : 0; !failed && i < tile; ++i)           // and the last products'
+            failed = !mbar_wait(bars + (L::kBarPv + (i & 3)) * 8, (i >> 2) & 1, abort_flag);
+    }
     if (failed && lane == 0) give_up(abort_flag, a.status, kStatusSoftmaxWait);
 }
 

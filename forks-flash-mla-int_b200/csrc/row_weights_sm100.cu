@@ -211,6 +211,11 @@ __device__ __forceinline__ void loader_role(const WeightsArgs &a, uint8_t *smem,
         }
         if (ok) ++tile_n;
     }
+    // What the products still signal to this CTA has to have come before it may end.
+    for (uint32_t i = st > static_cast<uint32_t>(L::kStages) ? st - L::kStages : 0; ok && i < st; ++i)
+        ok = mbar_wait(bars + (L::kBarEmpty + i % L::kStages) * 8, (i / L::kStages) & 1, abort_flag);
+    if (RES && tile_n > 0)
+        for (int s = 0; ok && s < a.k_slabs; ++s) ok = mbar_wait(bars + (L::kBarKEmpty + s) * 8, (tile_n - 1) & 1, abort_flag);
     if (!ok) {
         // The copies in flight have to land before the CTA may end.  Those of a pair are counted on the even CTA's barriers,
         // which wait for both CTAs' bytes; the odd one stays until the even one has seen them (cluster barrier at the end).
