@@ -9,7 +9,9 @@
 //
 // A cluster of CTAs takes a sequence.  Each holds its part of the keys in shared memory, so the weights are read
 // once, and the counts of a pass are added up through distributed shared memory.  What bounds it is latency: the
-// passes (two to four), each a count, a cluster barrier and a search, one after the other.  64 sequences of 32768 rows, two
+// passes (two to four), each a count, a cluster barrier and a search, one after the other, and in the first one adds that
+// wait for one another: the top eight bits of a key are the sign and seven bits of the exponent, of which such sums have a handful
+// (and zeros), so many lanes of a warp add to one word.  64 sequences of 32768 rows, two
 // CTAs each: 19 us, of which reading the weights (8 MB) would be 1.3; of 15 in the kernel the first pass takes 4, the second 3,
 // counting what stays 1.6 and writing it 4.5.  Four sequences of 2048 rows: 8 us back to back, 4 of them in the kernel.
 #include <cooperative_groups.h>
@@ -253,7 +255,8 @@ __device__ __forceinline__ int rows_to_move(const smla_compact_params_t &p, int 
 
 // Inside their own pages: a CTA takes 64 bytes of all rows of a sequence (slices of a row do not touch one another) and
 // moves 512 rows at a time, all their loads in front of all their stores.  A row's source index is at least its target's,
-// so what a later turn reads has not been written yet.  Bound by the latency of a turn, a load and a barrier.
+// so what a later turn reads has not been written yet.  Bound by the latency of a turn, three loads that depend on one another
+// and two barriers: 16 sequences x 4096 rows 55 us, one of 32768 rows 276 us (18 CTAs, 64 turns).
 constexpr int kSlice = 64, kTurnRows = 512;
 template <int THREADS>
 __device__ __forceinline__ void move_slice_in_place(const smla_compact_params_t &p, int b, int n, int slice) {
@@ -292,7 +295,7 @@ __global__ void __launch_bounds__(kSliceThreads) move_rows_in_place_kernel(const
 }
 
 // To other pages: a warp takes four rows, works out their addresses once and has all their pieces in flight together (three
-// of 16 bytes a lane and row: 1152 bytes are 2.25).  Bound by HBM, 2 x row_bytes a row.
+// of 16 bytes a lane and row: 1152 bytes are 2.25).  Bound by HBM, 2 x row_bytes a row: 16 sequences x 4096 rows 29 us, 5.2 TB/s.
 // A sequence whose target table names some of the source's pages in their own place (a copy of the table, or a table that
 // goes on with new pages) moves in place there: its rows are taken in order, by the first CTAs.
 constexpr int kMoveWarps = 8, kMoveRows = 4, kMoveTurn = 3;

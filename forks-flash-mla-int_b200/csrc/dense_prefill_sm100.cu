@@ -18,10 +18,11 @@
 // Three tiles are scored ahead of the output, so the weights of a tile have the time of two tiles' products to be computed
 // in, and two warpgroups take turns at the tiles: a weight computation (about 2100 cycles for a tile, one row per thread)
 // may take nearly twice as long as the products of a tile (1280 cycles at 192 dims).
-// What bounds it: tensor work, at 88 % while a long item runs (1400 cycles a tile: the chain weights - output - score of the
+// What bounds it: tensor work, at 91 % while a long item runs (1280 of 1400 cycles a tile: the chain weights - output - score of the
 // tile three on takes a little longer than three tiles' products), and the power limit in long runs.  From item to item the
-// output takes about 4000 cycles (last product, read, first product), of which half is hidden.  8192 causal tokens of 37
-// heads: 573 us with 192 dims (1.39 PFLOP/s), 502 us with 128 (1.27).  Measured against it: one CTA per item, S in one buffer
+// output takes about 4000 cycles (last product, read, first product), of which half is hidden: two tiles an item.  8192 causal tokens of 37
+// heads: 573 to 616 us with 192 dims, from GPU to GPU (1.39 to 1.29 PFLOP/s), 502 to 541 us with 128 (1.27 to 1.18).  Measured
+// against the former: one CTA per item, S in one buffer
 // for each half of the rows, 675 and 580 us; weights in buffers of their own beside S (a fourth wait and narrower stores)
 // 660 and 587; weights handed over in two pieces 602 and 530; the rows' reference through mbarriers in place of named ones
 // 600 and 542; the output written by the softmax warpgroup that had the last tile 577 and 509.

@@ -14,7 +14,7 @@
 //   C > 128 (a window)        pairs of CTAs that multiply as one (M = 256, half of the columns in each CTA's shared memory).
 //            The rows of a pair's tile stay in shared memory (147 KB each) while the columns pass in blocks of 256 through the
 //            ring; the next tile's slabs replace the rows as the last block leaves them.  With scratch the blocks of all tiles
-//            are dealt out evenly, and tiles that are cut are joined by a second kernel.  8192 columns, 28939 rows: 213 us, 1.28
+//            are dealt out evenly, and tiles that are cut are joined by a second kernel.  8192 columns, 28939 rows: 216 us, 1.26
 //            PFLOP/s (single CTAs with blocks of 128: 254 us).  Bound by the feed of columns: each pair takes 295 KB a block
 //            from L2, 6 TB/s over all.  (Eight stages of 8 KB in place of four of 16 KB: 5 % slower.)
 // Roles (384 threads): warps 0-3 and 4-7 take turns at the score blocks (two accumulators), warp 8 issues the MMAs, warp
@@ -64,10 +64,12 @@ struct WeightsArgs {
 // rounding; their signs vary (one sequence, 16 columns: 4.5e-6 -> 3e-7).
 // More: a score starts at B (the scale's sign), and after half of its steps 8/3 B is taken off, so that it goes on from -5/3 B.
 // B = 1.125 2^j, with 2^j times the scale between 8 and 16: for scores up to 7, which have the weight, the sum then stays
-// between 2^j and 2^(j+1) in size, and the errors of the halves are the same on average, with opposite signs.  What is left
-// of a score, 2.7e-6, varies from column to column and averages out in the sums (64 query positions of 128 heads: 3.7e-6 ->
-// 2.3e-7).  Scores of other sizes fare as without B.  Both offsets are products of their own, of constant operands: 38 steps
-// for 36.
+// between 2^j and 2^(j+1) in size, and the errors that a step's sum makes are the same in both halves on average, with opposite
+// signs.  What is left of a score, 2.7e-6, varies from column to column and averages out in the sums (64 query positions of 128
+// heads, all rows: 3.7e-6 -> 2.3e-7).  Not turned is what does not follow the sum's sign: a row that all queries look at, whose
+// products have one sign, stays 1.2e-6 to 1.6e-6 too light (64 to 512 columns, scores of 2 to 7, directions of random components),
+// 4e-6 where the components are all of one size.  Scores beyond 7 fare as without B.  Both offsets are products of their own, of
+// constant operands: 38 steps for 36.
 template <bool RES, int N>
 struct Smem {
     static constexpr bool kBalanced = N >= 64;

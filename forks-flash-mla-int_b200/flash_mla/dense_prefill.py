@@ -39,7 +39,9 @@ def dense_mla_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seql
     are copied first.
 
     Returns out (total_q, num_heads, 128) of q's type and softmax_lse (num_heads, total_q) float32, the natural
-    logarithm of the sum of exponentials.  A query that sees no key gets zeros and -inf; rows of q behind the
+    logarithm of the sum of exponentials.  Scores, sums and the output before its last rounding are fp32; the weights
+    are rounded to q's type for the second product, so out is up to 1.5 times as far from the exact value as one
+    rounding at the end would leave it.  A query that sees no key gets zeros and -inf; rows of q behind the
     last sequence are not written."""
     try:
         scale = q.shape[-1] ** (-0.5) if softmax_scale is None else float(softmax_scale)

@@ -232,7 +232,8 @@ SMLA_API int smla_dense_mla_prefill(const smla_prefill_params_t *params, void *s
  *      w[b, r] = sum over i, h with r visible to query i of exp(scale q[b, i, h, :] . K[b, r, :] - lse[b, h, i]).
  *    `accumulate` adds it to what `weights` holds for the rows of the sequence and leaves the others as they are;
  *    without it the whole [batch, weights_width] is written, 0 behind the sequence's rows.  A query whose lse is
- *    -inf gives nothing.  Sums are fp32 in a fixed order (two calls give the same bits; another workspace, another GPU
+ *    -inf gives nothing.  The tensor cores cut the sums of a score off toward zero: with more than 32 (position, head) pairs
+ *    a row that all queries look at may be lighter by 4e-6 of its weight, in proportion more for scores beyond 7.  Sums are fp32 in a fixed order (two calls give the same bits; another workspace, another GPU
  *    or other sequences beside a sequence may change the order).  A page number outside the cache is a page of zero
  *    rows, as in the decode.  One launch, with a workspace two. */
 typedef struct smla_row_weights_params {
